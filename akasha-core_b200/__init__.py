@@ -64,6 +64,8 @@ EmbeddingMeta = _u32struct("EmbeddingMeta", ["vocab_size", "dim", "seq_len"])
 FlashAttnMeta = _u32struct("FlashAttnMeta", ["seq_len", "dim", "head_dim", "scale", "row_offset"], floats=("scale",))
 AttnDecodeParams = _u32struct("AttnDecodeParams", ["rows", "heads", "head_dim", "block_size", "max_blocks_per_seq",
                                                    "scale", "kv_dtype", "n_splits", "pool_blocks"], floats=("scale",))
+AttnQ8Params = _u32struct("AttnQ8Params", ["rows", "q_len", "heads", "kv_heads", "head_dim", "block_size", "max_blocks_per_seq", "scale",
+                                           "dtype", "n_splits", "pool_blocks"], floats=("scale",))
 EngineConfig = _u32struct("EngineConfig", ["max_seqs", "max_seq_len", "kv_blocks", "block_size", "max_batch_tokens",
                                            "use_cuda_graph", "stop_on_eos", "attn_timing", "async_steps", "prefill_chunk_rows"])
 
@@ -122,6 +124,11 @@ _PROTOS = {
     "ak_transpose_to_bf16": [vp, vp, vp, C.c_uint32, C.c_uint32],
     "ak_f32_to_bf16": [vp, vp, vp, C.c_uint64],
     "ak_bf16_to_f32": [vp, vp, vp, C.c_uint64],
+    "ak_rmsnorm_q8": [vp, vp, C.c_uint32, vp, vp, vp, vp, NormMeta],
+    "ak_gemm_q8": [vp, vp, vp, vp, vp, vp, MatMulMeta, C.c_uint32, C.c_uint32],
+    "ak_rope_kv_append_q8": [vp, vp, vp, C.c_uint32, vp, vp, vp, vp, vp, vp, vp] + [C.c_uint32] * 7,
+    "ak_kv_read_q8": [vp, vp, vp, vp, vp, vp, vp, vp] + [C.c_uint32] * 6,
+    "ak_attn_decode_paged_q8": [vp, vp, vp, vp, vp, vp, vp, vp, vp, AttnQ8Params],
     "ak_ctx_create": [C.c_int, C.POINTER(vp)],
     "ak_ctx_destroy": [vp],
     "ak_ctx_synchronize": [vp],

@@ -85,6 +85,9 @@ int launch_gemm_bf16_argmax(cudaStream_t st, const void* a, const void* wt, floa
 int launch_argmax_finish(cudaStream_t st, const float* part_val, const uint32_t* part_idx, uint32_t rows, uint32_t tiles,
                          const int32_t* row_active, uint32_t* out_idx);
 
+// ---- gemm_q8.cu ----
+int gemm_q8_status(unsigned int* out);  // device status word of the 8-bit product
+
 // ---- attn_decode.cu ----------------------------------------------------------------------------
 size_t attn_decode_scratch_bytes(uint32_t rows, uint32_t heads, uint32_t head_dim, uint32_t n_splits);
 // counters_are_zero: the launch will not have to clear its arrival counters

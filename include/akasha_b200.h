@@ -272,6 +272,61 @@ AK_API int ak_transpose_to_bf16(void* stream, const float* w_kn, void* wt_nk, ui
 AK_API int ak_f32_to_bf16(void* stream, const float* src, void* dst, uint64_t n);
 AK_API int ak_bf16_to_f32(void* stream, const void* src, float* dst, uint64_t n);
 
+/* ---- 8-bit operators (no counterpart in the reference) ----
+ * A row of numbers y is held as int8 values q = rint(127 y / max|y|) in -127..127 and one f32 scale s = max|y| / 127: y ~ q s, off by at
+ * most s / 2. Rows are a token's activations, an output channel's weights, or one head's key or value at one cached position. A row whose
+ * largest magnitude is under 1e-30 is held as zeros with s = 0; one with an infinity or a NaN as zeros with s = NaN, so that whatever is
+ * computed from it is NaN. A call whose output (or, for the cache, key pool) lies on another device than the current one, or in memory that no
+ * kernel can reach, returns AK_ERR_INVALID_ARG; all buffers of a call belong on the same device. Nothing is kept between calls, no
+ * workspace is needed, and every call may be captured into a graph. Results do not depend on timing: the same call gives the same bits. */
+
+/* RMS norm with the residual's addition and an 8-bit result:
+ *   h = x + residual (residual != NULL: f32 x only; h is written back to x), y = h * rsqrt(mean(h^2) + eps) * w per row, q and scales as above.
+ *   w == NULL: y = h, the rows are quantised as they are (weights [n,k] for ak_gemm_q8, activations behind SiLU or attention).
+ * x [seq_len, size] f32 or bf16 (in_dtype); residual f32, w f32 [size]; q int8 [seq_len, size]; scales f32 [seq_len]. Any size; the
+ * fast form wants x and residual aligned to 4 elements and q to 4 bytes (any size), the others run element by element. */
+AK_API int ak_rmsnorm_q8(void* stream, void* x, uint32_t in_dtype, const float* residual, const float* w, int8_t* q, float* scales, ak_norm_meta m);
+
+/* 8-bit tensor-core product: C[m,n] (op)= (sum_k A[m,k] Wt[n,k]) * a_scales[m] * w_scales[n], A and Wt int8 row-major, sums exact in
+ * 32-bit integers, one f32 product with each scale, then the epilogue (ak_gemm_epilogue). ldc: row pitch of C in elements (>= n; as for
+ * ak_gemm_bf16_ld an odd width wants a padded pitch). k: a multiple of 16, 16 to 131056. A, Wt and C 16-byte aligned. A row's result is the same
+ * however many rows share the call. */
+AK_API int ak_gemm_q8(void* stream, const int8_t* a, const float* a_scales, const int8_t* wt, const float* w_scales, void* c, ak_matmul_meta m,
+                      uint32_t epilogue, uint32_t ldc);
+
+/* The 8-bit paged cache: k_pool, v_pool int8 [pool_blocks, kv_heads, 16, head_dim], k_scales, v_scales f32 [pool_blocks, kv_heads, 16],
+ * all 16-byte aligned; heads is a multiple of kv_heads, query head h reads kv head h / (heads / kv_heads). head_dim: 32, 64, 96 or 128.
+ * pool_blocks bounds what a call touches: a slot or block id outside the pool is never read or written.
+ *
+ * Fused head split + RoPE + quantisation + append: qkv [tokens, (heads + 2 kv_heads) * head_dim] f32 holds q | k | v of a token. q is rotated
+ * into q_out [tokens, heads * head_dim] (q_dtype); k is rotated, v kept as it is, and both are quantised into their slot (slots[t], -1 or outside
+ * the pool = not cached). rope_table as in ak_attn_decode_append_paged. A token whose position is outside [0, rope_len) is left out:
+ * nothing of it is written. No two tokens of a call may have the same slot. */
+AK_API int ak_rope_kv_append_q8(void* stream, const float* qkv, const float* rope_table, uint32_t rope_len, const int32_t* positions, const int32_t* slots,
+                                void* q_out, int8_t* k_pool, int8_t* v_pool, float* k_scales, float* v_scales, uint32_t tokens, uint32_t heads,
+                                uint32_t kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t q_dtype, uint32_t pool_blocks);
+/* Cached rows back as numbers: k_out, v_out [tokens, kv_heads * head_dim] (out_dtype; either may be NULL) = q s of slots[t], rounded once;
+ * zeros for a slot of -1 or outside the pool. Slots may repeat. (ak_flash_attention takes f32 rows read back like this.) */
+AK_API int ak_kv_read_q8(void* stream, const int8_t* k_pool, const int8_t* v_pool, const float* k_scales, const float* v_scales, const int32_t* slots,
+                         void* k_out, void* v_out, uint32_t tokens, uint32_t kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t out_dtype,
+                         uint32_t pool_blocks);
+/* Attention of the newest q_len tokens of every sequence over the cache (decode: q_len = 1; drafted tokens or a chunk of a prompt: more):
+ *   q, out [rows * q_len, heads * head_dim] (dtype); query i of a row is at position kv_lens[row] - q_len + i and sees the positions up to its
+ *   own (kv_lens counts the new tokens, which are in the cache already). Lengths are cut at 16 * max_blocks_per_seq; a query with no
+ *   position to see gives zeros. block_tables int32 [rows, max_blocks_per_seq], entries past a sequence's end are not read; the positions of a block id
+ *   outside the pool are left out. scale multiplies q . k.
+ *   n_splits: CTAs that share a sequence, as one thread-block cluster; 0 = the library's choice, else 1 to 16 (rounded down to a power of two).
+ * f32 arithmetic throughout (queries and softmax weights as two f16 parts), but for bf16 with more than 8 query rows per kv head
+ * (q_len * heads / kv_heads), where weights are rounded to f16. A weight below 2^-38 of its sequence's largest weight-times-scale may count as 0. */
+typedef struct ak_attn_q8_params {
+    uint32_t rows, q_len, heads, kv_heads, head_dim, block_size, max_blocks_per_seq;
+    float scale;
+    uint32_t dtype; /* ak_dtype of q and out */
+    uint32_t n_splits, pool_blocks;
+} ak_attn_q8_params;
+AK_API int ak_attn_decode_paged_q8(void* stream, const void* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scales, const float* v_scales,
+                                   const int32_t* block_tables, const int32_t* kv_lens, void* out, ak_attn_q8_params p);
+
 /* ================================================================== 2. session level */
 typedef struct ak_ctx ak_ctx;         /* one device + one stream (Arc<B: Backend>) */
 typedef struct ak_weights ak_weights; /* ModelWeights (src/nn/weights.rs:40-47)     */

@@ -55,6 +55,22 @@ pub struct AkAttnDecodeParams {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct AkAttnQ8Params {
+    pub rows: u32,
+    pub q_len: u32,
+    pub heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub block_size: u32,
+    pub max_blocks_per_seq: u32,
+    pub scale: f32,
+    pub dtype: u32,
+    pub n_splits: u32,
+    pub pool_blocks: u32,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct AkEngineConfig {
     pub max_seqs: u32,
@@ -161,6 +177,22 @@ extern "C" {
     pub fn ak_transpose_to_bf16(stream: Stream, w_kn: *const f32, wt_nk: *mut c_void, k: u32, n: u32) -> c_int;
     pub fn ak_f32_to_bf16(stream: Stream, src: *const f32, dst: *mut c_void, n: u64) -> c_int;
     pub fn ak_bf16_to_f32(stream: Stream, src: *const c_void, dst: *mut f32, n: u64) -> c_int;
+
+    // ---- 8-bit operators: int8 rows with f32 scales
+    pub fn ak_rmsnorm_q8(stream: Stream, x: *mut c_void, in_dtype: u32, residual: *const f32, w: *const f32, q: *mut i8, scales: *mut f32,
+                         m: NormMeta) -> c_int;
+    pub fn ak_gemm_q8(stream: Stream, a: *const i8, a_scales: *const f32, wt: *const i8, w_scales: *const f32, c: *mut c_void, m: MatMulMeta,
+                      epilogue: u32, ldc: u32) -> c_int;
+    pub fn ak_rope_kv_append_q8(stream: Stream, qkv: *const f32, rope_table: *const f32, rope_len: u32, positions: *const i32,
+                                slots: *const i32, q_out: *mut c_void, k_pool: *mut i8, v_pool: *mut i8, k_scales: *mut f32,
+                                v_scales: *mut f32, tokens: u32, heads: u32, kv_heads: u32, head_dim: u32, block_size: u32, q_dtype: u32,
+                                pool_blocks: u32) -> c_int;
+    pub fn ak_kv_read_q8(stream: Stream, k_pool: *const i8, v_pool: *const i8, k_scales: *const f32, v_scales: *const f32,
+                         slots: *const i32, k_out: *mut c_void, v_out: *mut c_void, tokens: u32, kv_heads: u32, head_dim: u32,
+                         block_size: u32, out_dtype: u32, pool_blocks: u32) -> c_int;
+    pub fn ak_attn_decode_paged_q8(stream: Stream, q: *const c_void, k_pool: *const i8, v_pool: *const i8, k_scales: *const f32,
+                                   v_scales: *const f32, block_tables: *const i32, kv_lens: *const i32, out: *mut c_void,
+                                   p: AkAttnQ8Params) -> c_int;
 
     // ---- context, tensor parallelism, weights (`ModelWeights::params()` order, src/nn/weights.rs:158-171)
     pub fn ak_ctx_create(device: c_int, out: *mut *mut AkCtx) -> c_int;
