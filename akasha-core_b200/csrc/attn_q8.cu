@@ -5,19 +5,30 @@
 // k_j, v_j are int8 rows, ks_j, vs_j their f32 scales. One pass over the cache with the running maximum and sum of the softmax; the
 // bytes of the cache are read once and bound the kernel (132 bytes per position and kv head at head size 64, 264 at 128).
 //
-// The products run on mma.sync.m16n8k16 in f16: int8 is exact in f16 (1024 + 128 + v is assembled by a byte permute and 1152 taken off),
-// and the tile of 16 rows is one more than a group of query heads fills: decode has one query per (sequence, head), so tcgen05, whose
-// smallest tile is 64 rows of one K, has nothing to work with. The rows of the A operand:
-//   PIECES = 2: 8 queries, rows 0-7 their leading f16 part and rows 8-15 what is left of it (22 bits together), for q and for the
-//               weights p * vs alike. Both f32 and bf16 results come out as from f32 arithmetic, and for up to 8 query rows it costs nothing:
-//               the other 8 rows would be empty.
-//   PIECES = 1: 16 queries (bf16 results, more than 8 query rows per kv head): weights rounded once to f16 (2^-12, the result to 2^-9).
-// q is scaled by a power of two per row to below 2^15, the weights by one that follows the largest value scale met so far (below 2^14), so
-// that f16's range does not matter: a leading part's last bit is 2^-10 of its value, down to 2^-38 of the largest one.
+// Decode has one query per (sequence, head), a group of heads or a few drafted tokens at most 16 or so: tcgen05, whose smallest tile is 64
+// rows of one K, has nothing to work with, and mma.sync takes the cache as its 16-row operand, the queries as the 8-column one. A column pair
+// is one query in two parts, so that the 8 columns are 4 queries:
+//   S^T = K q   m16n8k32 on int8 as it lies in the cache. A query is held as integers X = rint(q F), F = 127 * 256^(D - 1) / max|q|, in
+//               D signed base-256 digits: 2 for bf16 (16 bits of the head's largest value), 3 for f32 (24 bits). Sums of digits are exact.
+//   O^T = V p   m16n8k16 on f16, in which int8 is exact (1024 + 128 + v is put together by a byte permute and 1152 taken off). A weight
+//               w = p vs is its leading f16 part and what is left of it (22 bits together, TWO), or, for bf16 results and more than 4 query
+//               rows, the leading part alone (11 bits; the result has 8) with two queries to a column pair.
+// Scores come out with lanes holding positions g, g + 8 of one query, and turn into the second product's operand by a transposition of 8 x 8
+// blocks (movmatrix). With the queries as the 16-row operand of f16 products (and keys converted like values) a tile took 370 instructions and 168
+// registers instead of 280 and 122, and 64 x 16 heads x 2048 positions x 128 113 us instead of 86.
 //
-// A CTA of WARPS warps takes one (sequence, kv head, tile of queries, split); each warp has every WARPS-th cache block of the split and a
-// ring of cp.async stages of its own, no barrier in the loop. The warps' results are merged in shared memory and the splits', which are
-// the CTAs of one cluster, through distributed shared memory in split order: no scratch, no atomics, the same bits every time.
+// Weights are 2^(s - m) with a reference m that follows the running maximum only when a score is more than 8 above it: up to then weights
+// grow to 2^8, which f16 has room for (they are scaled by a power of two, below 2^13, that follows the largest value scale met so far), and no
+// reduction over the lanes stands between the two products.
+//
+// Measured (graph of launches on three sets of inputs, cold L2): 64 sequences x 16 heads x 128, 64 to 4096 positions 90 us = 0.96 of the copy
+// bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 24 us = 0.68: bound by instructions there (231 a tile of 2176 bytes, issue
+// slots 72 % busy); 2 sequences of 60000 x 8 kv heads x 16 query rows 63 us = 0.59: few CTAs, instructions; one sequence of 300 x 5 heads
+// 5.8 us, a chain of latencies (an empty launch takes 2).
+//
+// A CTA takes one (sequence, kv head, tile of queries, split); each warp has every n-th cache block of the split and a ring of cp.async
+// stages of its own, no barrier in the loop. The warps' results are merged in shared memory and the splits', which are the CTAs of one
+// cluster, through distributed shared memory in split order: no scratch, no atomics, the same bits every time.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -28,16 +39,15 @@ namespace cg = cooperative_groups;
 
 namespace ak {
 
-constexpr int AQ_WARPS = 4;
+constexpr uint32_t AQ_MAX_WARPS = 8;
 constexpr uint32_t AQ_MAX_SPLITS = 16;   // CTAs of a cluster (8 is the portable limit, 16 is asked for)
 
 template <int HD> struct AqCfg {
     static constexpr int TILE = 16 * HD;                   // bytes of a block's keys (or values) of one head
     static constexpr int STAGE = 2 * TILE + 128;           // keys | values | 16 key scales | 16 value scales
-    static constexpr int STAGES = HD >= 96 ? 3 : 4;
-    static constexpr int RING = AQ_WARPS * STAGES * STAGE;
+    static constexpr int STAGES = HD == 128 ? 3 : 4;       // of a warp's ring (3, 4 and 6 are the same to a microsecond at 128: latency is not what bounds it)
+    static constexpr int CTAS = HD >= 96 ? 2 : 3;          // of AQ_MAX_WARPS warps that an SM holds: 16 warps (128 registers), 24 (80) up to head size 64
 };
-
 // Where 16-byte chunk `col` of row `row` sits in a tile. Keys are read 4 chunks of 2 rows at a time, values 32 bytes of every other row:
 // the permutations keep either within distinct banks (head sizes 64 and 128; 96 has two-way conflicts).
 template <int HD> __device__ __forceinline__ uint32_t k_at(uint32_t row, uint32_t col) {
@@ -66,9 +76,9 @@ template <int N> __device__ __forceinline__ void lds_words(uint32_t a, uint32_t*
     else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
     else w[0] = lds32(a);
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t a) {
-    float2 v;
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+__device__ __forceinline__ float lds_f(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
     return v;
 }
 
@@ -83,8 +93,24 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float2 unpack_half2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
+// D(16x8, s32) += A(16x32, s8, row) B(32x8, s8, col)
+__device__ __forceinline__ void mma_s8(int32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_first(int32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+// the transpose of the 8 x 8 block of which lane (g, t) holds row g, columns 2t and 2t + 1
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
 // D(16x8, f32) += A(16x16, f16, row) B(16x8, f16, col)
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -108,387 +134,505 @@ struct AqArgs {
     float scale;
 };
 
-// The d-index of word w (4 consecutive values) that lane t of a quad holds of a key row: chunk t, then chunk 4 + t (HD 128), 8-byte pieces for
-// what is left. The order in which q . k is summed is free as long as q is laid out alike.
+// The d-index of word w (4 consecutive values) that lane t of a quad holds of a key row: chunk t, then chunk 4 + t (HD 128), an 8-byte piece
+// where there are no four chunks. The order in which q . k is summed is free as long as q is laid out alike.
 template <int HD> __device__ __forceinline__ uint32_t d_of(uint32_t t, int w) {
     if (HD == 32) return 8 * t + 4 * w;
     if (w < 4) return 16 * t + 4 * w;
     if (HD == 96) return 64 + 8 * t + 4 * (w - 4);
     return 64 + 16 * t + 4 * (w - 4);
 }
-template <int HD> __device__ __forceinline__ void load_key(uint32_t tile, uint32_t row, uint32_t t, uint32_t (&w)[HD / 16]) {
-    if constexpr (HD == 32) {
-        lds_words<2>(tile + row * 32 + 8 * t, w);
-    } else {
-        lds_words<4>(tile + k_at<HD>(row, t), w);
-        if constexpr (HD == 128) lds_words<4>(tile + k_at<HD>(row, 4 + t), w + 4);
-        if constexpr (HD == 96) lds_words<2>(tile + row * 96 + 64 + 8 * t, w + 4);
+// A lane's offsets in a tile, the same for every tile. 8 rows further is 8 HD bytes further whatever the permutation.
+template <int HD> struct AqLane {
+    uint32_t key, key2;       // its first chunk of row g, and its second piece
+    uint32_t val, val2;       // its HD / 8 values of rows 2t and 2t + 1
+    uint32_t put_k, put_v;    // where it puts the first 16 bytes that it copies
+    __device__ __forceinline__ AqLane(uint32_t lane) {
+        const uint32_t g = lane >> 2, t = lane & 3, row = lane / (HD / 16), col = lane % (HD / 16);
+        key = HD == 32 ? g * 32 + 8 * t : k_at<HD>(g, t);
+        key2 = HD == 128 ? k_at<HD>(g, 4 + t) : g * HD + 64 + 8 * t;
+        const uint32_t byte = (HD / 8) * g;
+        val = HD == 128 || HD == 64 ? v_at<HD>(2 * t, byte >> 4) + (byte & 15) : 2 * t * HD + byte;
+        val2 = HD == 128 || HD == 64 ? v_at<HD>(2 * t + 1, byte >> 4) + (byte & 15) : (2 * t + 1) * HD + byte;
+        put_k = k_at<HD>(row, col);
+        put_v = v_at<HD>(row, col);
     }
-}
-// The HD / 8 values from HD / 8 * g on of a value row
-template <int HD> __device__ __forceinline__ void load_value(uint32_t tile, uint32_t row, uint32_t g, uint32_t (&w)[HD / 32]) {
-    if constexpr (HD == 128) lds_words<4>(tile + v_at<128>(row, g), w);
-    else if constexpr (HD == 64) lds_words<2>(tile + v_at<64>(row, g >> 1) + ((g & 1) << 3), w);
-    else if constexpr (HD == 32) w[0] = lds32(tile + row * 32 + 4 * g);
-    else {
+    __device__ __forceinline__ void load_key(uint32_t tile, uint32_t (&w)[HD / 16]) const {
+        if constexpr (HD == 32) lds_words<2>(tile + key, w);
+        else lds_words<4>(tile + key, w);
+        if constexpr (HD == 128) lds_words<4>(tile + key2, w + 4);
+        if constexpr (HD == 96) lds_words<2>(tile + key2, w + 4);
+    }
+    __device__ __forceinline__ void load_value(uint32_t at, uint32_t (&w)[HD / 32]) const {
+        if constexpr (HD == 96) {
 #pragma unroll
-        for (int i = 0; i < 3; i++) w[i] = lds32(tile + row * 96 + 12 * g + 4 * i);
+            for (int i = 0; i < 3; i++) w[i] = lds32(at + 4 * i);
+        } else {
+            lds_words<HD / 32>(at, w);
+        }
     }
-}
+};
 
-template <typename T, int HD, int PIECES>
-__global__ void __launch_bounds__(AQ_WARPS * 32)
+template <typename T, int HD, int NQ, bool TWO>
+__global__ void __launch_bounds__(AQ_MAX_WARPS * 32, AqCfg<HD>::CTAS)
 attn_decode_q8_kernel(const AqArgs a) {
     using C = AqCfg<HD>;
-    constexpr int ROWS = PIECES == 2 ? 8 : 16;    // queries of a tile
-    constexpr int NR = PIECES == 2 ? 1 : 2;       // of them a lane holds
-    constexpr int KW = HD / 16;                   // words of a key row per lane = steps of q . k
-    constexpr int NT = HD / 8;                    // 8-wide tiles of the result
-    constexpr bool LOW_Q = PIECES == 2 && sizeof(T) == 4;   // bf16 queries have no second part (8 bits)
-    constexpr bool HIGH_ROWS_Q = PIECES == 1 || LOW_Q;
+    constexpr int STAGES = C::STAGES;
+    constexpr int ROWS = 4 * NQ;                     // queries of a tile: NQ column blocks of 4
+    constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;   // of a query
+    constexpr int KW = HD / 16, KS = HD / 32;        // words of a key row per lane, steps of K q
+    constexpr int NP = TWO ? NQ : NQ / 2;            // column blocks of V p
+    constexpr int MT = HD / 16;                      // 16-row tiles of the result
     pdl_wait();
     pdl_trigger();
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float s_m[AQ_WARPS][ROWS], s_l[AQ_WARPS][ROWS];
-    __shared__ float s_top[ROWS], s_sum[ROWS];
+    __shared__ float s_m[AQ_MAX_WARPS][ROWS], s_l[AQ_MAX_WARPS][ROWS];
+    __shared__ float s_f[AQ_MAX_SPLITS][ROWS];            // factors of the warps' (then of the splits') results
+    __shared__ float s_top[AQ_MAX_SPLITS][ROWS], s_sum[AQ_MAX_SPLITS][ROWS], s_unit[ROWS];
+    __shared__ uint64_t s_at[ROWS];                       // where a row's query and result begin
+    __shared__ __align__(16) int8_t s_q[ROWS][DIGITS == 3 ? 4 : 2][HD];   // digits, the last plane of four is zero
 
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t qt = blockIdx.x % a.q_tiles, kvh = (blockIdx.x / a.q_tiles) % a.kv_heads, seq = blockIdx.x / (a.q_tiles * a.kv_heads);
     const uint32_t split = blockIdx.z, n_splits = gridDim.z;
     const uint32_t total_rows = a.q_len * a.group;
     const int32_t cap = (int32_t)(a.max_blocks * Q8_BS);
+    const int32_t* table = a.tables + (size_t)seq * a.max_blocks;
+    // Lane j: the cache block of this warp's tile (i & ~31) + j. Without splits the first ones are known before the length is.
+    uint32_t ids = 0xffffffffu;
+    if (n_splits == 1 && warp + lane * warps < a.max_blocks) ids = (uint32_t)table[warp + lane * warps];
     const int32_t len = a.lens[seq];
+    // The first queries are on their way while the length is.
+    constexpr int QV = HD / 8;       // values of a row that a thread takes, 8 threads a row
+    uint32_t qraw[QV * (int)sizeof(T) / 4];
+    auto q_row = [&](uint32_t r) -> uint64_t {   // where row r's query and result begin (row 0's for a row that is not there)
+        const uint32_t rr = qt * ROWS + r < total_rows ? qt * ROWS + r : qt * ROWS;
+        return (((uint64_t)seq * a.q_len + rr / a.group) * a.heads + (uint64_t)kvh * a.group + rr % a.group) * HD;
+    };
+    auto q_load = [&](uint64_t at) {
+        const uint8_t* qp = reinterpret_cast<const uint8_t*>(a.q) + at * sizeof(T);
+        if constexpr (QV * sizeof(T) % 16 == 0) {
+#pragma unroll
+            for (int e = 0; e < QV * (int)sizeof(T) / 16; e++) {
+                const uint4 v = reinterpret_cast<const uint4*>(qp)[e];
+                qraw[4 * e] = v.x; qraw[4 * e + 1] = v.y; qraw[4 * e + 2] = v.z; qraw[4 * e + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < QV * (int)sizeof(T) / 8; e++) {
+                const uint2 v = reinterpret_cast<const uint2*>(qp)[e];
+                qraw[2 * e] = v.x; qraw[2 * e + 1] = v.y;
+            }
+        }
+    };
+    uint64_t my_at = 0;
+    if (threadIdx.x < ROWS * 8) { my_at = q_row(threadIdx.x >> 3); q_load(my_at + (threadIdx.x & 7) * QV); }
 
-    // positions that row r of the tile may see
+
+    // ---- positions that row r of the tile may see
     auto limit_of = [&](uint32_t r) -> int32_t {
         const uint32_t rr = qt * ROWS + r;
         if (rr >= total_rows) return 0;
         const int64_t lim = (int64_t)len - a.q_len + rr / a.group + 1;
         return lim < 0 ? 0 : (int32_t)(lim < cap ? lim : cap);
     };
-    auto q_index = [&](uint32_t r) -> size_t {   // first value of row r's query (and result)
-        const uint32_t rr = qt * ROWS + r;
-        return (((size_t)seq * a.q_len + rr / a.group) * a.heads + (size_t)kvh * a.group + rr % a.group) * HD;
-    };
     const uint32_t last = min((uint32_t)ROWS, total_rows - qt * ROWS) - 1;
     const int32_t lim_min = limit_of(0), lim_max = limit_of(last);   // limits grow with the row
-    int32_t lim[NR];
+    int32_t lim[NQ];
 #pragma unroll
-    for (int r = 0; r < NR; r++) lim[r] = limit_of(g + 8 * r);
+    for (int u = 0; u < NQ; u++) lim[u] = limit_of(4 * u + t);
 
-    // ---- queries: A operand rows g (and g + 8), scaled to below 2^15 by a power of two
-    uint32_t qa[KW][HIGH_ROWS_Q ? 4 : 2];
-    float row_scale[NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const bool have = qt * ROWS + g + 8 * r < total_rows;
-        const T* qp = reinterpret_cast<const T*>(a.q) + (have ? q_index(g + 8 * r) : 0);
-        float x[KW][4];
-        uint32_t top = 0;
-#pragma unroll
-        for (int w = 0; w < KW; w++) {
-            const uint32_t d = d_of<HD>(t, w);
-            if constexpr (sizeof(T) == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(qp + d);
-                x[w][0] = v.x; x[w][1] = v.y; x[w][2] = v.z; x[w][3] = v.w;
-            } else {
-                const uint2 v = *reinterpret_cast<const uint2*>(qp + d);
-                x[w][0] = __uint_as_float(v.x << 16); x[w][1] = __uint_as_float(v.x & 0xffff0000u);
-                x[w][2] = __uint_as_float(v.y << 16); x[w][3] = __uint_as_float(v.y & 0xffff0000u);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (!have) x[w][e] = 0.0f;
-                top = max(top, abs_bits(x[w][e]));
-            }
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int e = (int)(top >> 23) - 127;              // floor(log2 max|q|)
-        const bool finite = top < 0x7f800000u;
-        const int ef = 13 - (e < -100 ? -100 : e);   // q * 2^ef is below 2^14
-        const float f = pow2i(finite ? ef : 0);
-        // scores in the base-2 domain; a query with an infinity or a NaN has NaN for every score
-        row_scale[r] = finite ? a.scale * 1.4426950408889634f * pow2i(-ef) : __uint_as_float(0x7fc00000u);
-#pragma unroll
-        for (int w = 0; w < KW; w++) {
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = finite ? x[w][i] * f : 0.0f;
-            const uint32_t h0 = pack_half2(y[0], y[1]), h1 = pack_half2(y[2], y[3]);
-            if (r == 0) { qa[w][0] = h0; qa[w][1] = h1; }
-            else { qa[w][HIGH_ROWS_Q ? 2 : 0] = h0; qa[w][HIGH_ROWS_Q ? 3 : 0] = h1; }
-            if constexpr (LOW_Q) {
-                const float2 b0 = unpack_half2(h0), b1 = unpack_half2(h1);
-                qa[w][2] = pack_half2(y[0] - b0.x, y[1] - b0.y);
-                qa[w][3] = pack_half2(y[2] - b1.x, y[3] - b1.y);
-            }
-        }
-    }
-
+    if (n_splits > 1) cluster_arrive_all();   // "this CTA runs", waited for before the first access to a peer
     // ---- this split's blocks, this warp's share of them
     const uint32_t nblk = ((uint32_t)lim_max + Q8_BS - 1) / Q8_BS;
     const uint32_t per = (nblk + n_splits - 1) / n_splits;
     const uint32_t b_begin = min(split * per, nblk), b_end = min(b_begin + per, nblk);
     const uint32_t first = b_begin + warp;
-    const uint32_t mine = first < b_end ? (b_end - first + AQ_WARPS - 1) / AQ_WARPS : 0;
-    const int32_t* table = a.tables + (size_t)seq * a.max_blocks;
-    const uint32_t ring = smem_u32(smem) + warp * (C::STAGES * C::STAGE);
+    const uint32_t mine = first < b_end ? (b_end - first + warps - 1) / warps : 0;
+    const uint32_t ring = smem_u32(smem) + warp * (STAGES * C::STAGE);
 
-    uint32_t ids = 0xffffffffu;   // lane j: the cache block of this warp's tile (i & ~31) + j
-    auto request = [&](uint32_t i) {
-        if (i < mine) {
-            if ((i & 31u) == 0) ids = i + lane < mine ? (uint32_t)table[first + (i + lane) * AQ_WARPS] : 0xffffffffu;
-            const uint32_t blk = __shfl_sync(0xffffffffu, ids, i & 31u);
+    // The next tile is asked for, into the next stage of the ring. A block outside the pool holds no positions: bit j of `there` says whether the
+    // j-th newest tile is there.
+    const AqLane<HD> at_lane(lane);
+    const int8_t *my_k = a.k_pool + lane * 16, *my_v = a.v_pool + lane * 16;
+    const float* my_s = (lane < 4 ? a.k_scales : a.v_scales) + (lane & 3) * 4;
+    uint32_t there = 0, asked = 0, put = ring;
+    auto request = [&]() {
+        there <<= 1;
+        if (asked < mine) {
+            if ((asked & 31u) == 0 && (asked > 0 || n_splits > 1)) ids = asked + lane < mine ? (uint32_t)table[first + (asked + lane) * warps] : 0xffffffffu;
+            const uint32_t blk = __shfl_sync(0xffffffffu, ids, asked & 31u);
+            asked++;
             if (blk < a.pool_blocks) {
-                const uint32_t dst = ring + (i % C::STAGES) * C::STAGE;
-                const size_t at = (size_t)blk * a.kv_heads + kvh;
-                const int8_t *ks = a.k_pool + at * C::TILE, *vs = a.v_pool + at * C::TILE;
+                there |= 1u;
+                const uint64_t at = (uint64_t)blk * a.kv_heads + kvh;
+                const int8_t *ks = my_k + at * C::TILE, *vs = my_v + at * C::TILE;
 #pragma unroll
-                for (uint32_t j = 0; j < (uint32_t)HD; j += 32) {
-                    const uint32_t c = j + lane, row = c / (HD / 16), col = c % (HD / 16);
-                    cp_async16(dst + k_at<HD>(row, col), ks + c * 16);
-                    cp_async16(dst + C::TILE + v_at<HD>(row, col), vs + c * 16);
+                for (int j = 0; j < HD / 32; j++) {
+                    cp_async16(put + at_lane.put_k + 512 * j, ks + 512 * j);
+                    cp_async16(put + C::TILE + (HD == 128 ? at_lane.put_v ^ ((j & 1) << 6) : at_lane.put_v) + 512 * j, vs + 512 * j);
                 }
-                if (lane < 8) cp_async16(dst + 2 * C::TILE + lane * 16, (lane < 4 ? a.k_scales : a.v_scales) + at * Q8_BS + (lane & 3) * 4);
+                if (lane < 8) cp_async16(put + 2 * C::TILE + lane * 16, my_s + at * Q8_BS);
             }
         }
+        put = put == ring + (STAGES - 1) * C::STAGE ? ring : put + C::STAGE;
         cp_commit();
     };
-    // Which tiles were requested: a block outside the pool holds no positions. (The ids of tile i are still in the window of tile i + STAGES
-    // only while both share a group of 32, so validity travels as a bit.)
-    uint32_t valid_bits = 0;
-    auto request_at = [&](uint32_t i) {
-        request(i);
-        const bool ok = i < mine && __shfl_sync(0xffffffffu, ids, i & 31u) < a.pool_blocks;
-        valid_bits = (valid_bits & ~(1u << (i % C::STAGES))) | ((ok ? 1u : 0u) << (i % C::STAGES));
-    };
 #pragma unroll
-    for (uint32_t i = 0; i + 1 < (uint32_t)C::STAGES; i++) request_at(i);
+    for (uint32_t i = 0; i + 1 < (uint32_t)STAGES; i++) request();
 
-    float m_run[NR], l_run[NR];
+    // ---- queries: digits into shared memory, for every warp
+    for (uint32_t i = threadIdx.x; i < ROWS * 8; i += blockDim.x) {   // whole groups of 8: blockDim.x and ROWS * 8 are multiples of 32
+        const uint32_t r = i >> 3, d = (i & 7) * QV;
+        const bool have = qt * ROWS + r < total_rows;
+        if (i >= blockDim.x) { my_at = q_row(r); q_load(my_at + d); }
+        float x[QV];
+        uint32_t top = 0;
 #pragma unroll
-    for (int r = 0; r < NR; r++) { m_run[r] = -INFINITY; l_run[r] = 0.0f; }
-    float acc[NT][4];
+        for (int e = 0; e < QV; e++) {
+            if constexpr (sizeof(T) == 4) x[e] = __uint_as_float(qraw[e]);
+            else x[e] = __uint_as_float((e & 1) ? qraw[e / 2] & 0xffff0000u : qraw[e / 2] << 16);
+            top = max(top, abs_bits(x[e]));
+        }
 #pragma unroll
-    for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-    int v_exp = -110;   // weights are p * vs * 2^(13 - v_exp), v_exp >= log2 of every finite value scale so far
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (!have) top = 0;
+        // |q| under 1e-30 counts as 0 (F would overflow); a query with an infinity or a NaN has NaN for every score
+        const float most = __uint_as_float(top), full = DIGITS == 3 ? 8323072.0f : 32512.0f;   // 127 * 256^(D - 1)
+        const bool finite = top < 0x7f800000u, some = finite && most >= Q8_ZERO;
+        const float F = some ? full / most : 0.0f;
+        if ((i & 7) == 0) {
+            s_unit[r] = !finite ? __uint_as_float(0x7fc00000u) : some ? most / full * (a.scale * 1.4426950408889634f) : 0.0f;   // scores in the base-2 domain
+            s_at[r] = my_at;
+        }
+#pragma unroll
+        for (int e = 0; e < QV; e += 4) {
+            uint32_t dg[3] = {0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                int32_t X = some ? __float2int_rn(x[e + j] * F) : 0;
+                // signed digits: the low byte as it is, what is left a multiple of 256
+#pragma unroll
+                for (int k = DIGITS - 1; k > 0; k--) {
+                    const int32_t low = (int8_t)X;
+                    dg[k] |= ((uint32_t)low & 0xffu) << (8 * j);
+                    X = (X - low) >> 8;
+                }
+                dg[0] |= ((uint32_t)X & 0xffu) << (8 * j);
+            }
+#pragma unroll
+            for (int k = 0; k < DIGITS; k++) *reinterpret_cast<uint32_t*>(&s_q[r][k][d + e]) = dg[k];
+            if constexpr (DIGITS == 3) *reinterpret_cast<uint32_t*>(&s_q[r][3][d + e]) = 0;
+        }
+    }
+    __syncthreads();
+    // operand lane (g, t): column g = digit g & 1 of query g >> 1 of each block (3 digits: of a second block, digits 2 and the zeros)
+    uint32_t qb[NQ][KS][DIGITS == 3 ? 4 : 2];
+    float row_scale[NQ];
+#pragma unroll
+    for (int u = 0; u < NQ; u++) {
+        row_scale[u] = s_unit[4 * u + t];
+#pragma unroll
+        for (int w = 0; w < KW; w++)
+#pragma unroll
+            for (int k = 0; k < (DIGITS == 3 ? 2 : 1); k++)
+                qb[u][w >> 1][2 * k + (w & 1)] = *reinterpret_cast<const uint32_t*>(&s_q[4 * u + (g >> 1)][2 * k + (g & 1)][d_of<HD>(t, w)]);
+    }
+
+    float m_ref[NQ], l_run[NQ];
+#pragma unroll
+    for (int u = 0; u < NQ; u++) {
+        const bool sees = lim[u] > 0;   // one that does not never asks for a reference
+        m_ref[u] = sees ? -INFINITY : 0.0f;
+        if (!sees) row_scale[u] = 0.0f;
+        l_run[u] = 0.0f;
+    }
+    uint32_t get = ring;
+    int32_t pos0 = (int32_t)(first * Q8_BS);
+    float acc[NP][MT][4];
+#pragma unroll
+    for (int u = 0; u < NP; u++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.0f;
+    int v_exp = -110;   // weights are p * vs * 2^(5 - v_exp) with vs < 2^v_exp for every finite value scale so far
 
     for (uint32_t i = 0; i < mine; i++) {
-        request_at(i + C::STAGES - 1);
-        cp_wait<C::STAGES - 1>();
+        request();
+        cp_wait<STAGES - 1>();
         __syncwarp();
-        if ((valid_bits >> (i % C::STAGES)) & 1u) {
-            const uint32_t ksm = ring + (i % C::STAGES) * C::STAGE, vsm = ksm + C::TILE, sks = vsm + C::TILE, svs = sks + 64;
-            const int32_t pos0 = (int32_t)((first + i * AQ_WARPS) * Q8_BS);
-            // ---- S = q . K^T: columns 2t, 2t + 1 of positions 0-7 and 8-15
-            float sc[2][4];
+        if (there & (1u << (STAGES - 1))) {
+            const uint32_t ksm = get, vsm = get + C::TILE, sks = get + 2 * C::TILE + 4 * g;
+            // ---- S^T = K q: positions g, g + 8 of query t
+            int32_t dot[NQ][DIGITS == 3 ? 2 : 1][4];
+            {
+                uint32_t k0[KW], k1[KW];
+                at_lane.load_key(ksm, k0);
+                at_lane.load_key(ksm + 8 * HD, k1);
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
-                uint32_t w[KW];
-                load_key<HD>(ksm, 8 * n + g, t, w);
+                for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int k = 0; k < KW; k++) {
-                    const uint32_t u = w[k] ^ 0x80808080u;
-                    const uint32_t b0 = half2_of(u, 0x4140), b1 = half2_of(u, 0x4342);
-                    if constexpr (HIGH_ROWS_Q) mma_f16(sc[n], qa[k][0], qa[k][2], qa[k][1], qa[k][3], b0, b1);
-                    else mma_f16(sc[n], qa[k][0], 0u, qa[k][1], 0u, b0, b1);
-                }
+                    for (int u = 0; u < NQ; u++) {
+#pragma unroll
+                        for (int d = 0; d < (DIGITS == 3 ? 2 : 1); d++) {
+                            if (k == 0) mma_s8_first(dot[u][d], k0[0], k1[0], k0[1], k1[1], qb[u][0][2 * d], qb[u][0][2 * d + 1]);
+                            else mma_s8(dot[u][d], k0[2 * k], k1[2 * k], k0[2 * k + 1], k1[2 * k + 1], qb[u][k][2 * d], qb[u][k][2 * d + 1]);
+                        }
+                    }
             }
-            const float2 ka = lds_f2(sks + 8 * t), kb = lds_f2(sks + 32 + 8 * t);
-            const float2 va = lds_f2(svs + 8 * t), vb = lds_f2(svs + 32 + 8 * t);
-            const float kscale[4] = {ka.x, ka.y, kb.x, kb.y};
-            float vscale[4] = {va.x, va.y, vb.x, vb.y};
+            const float ka = lds_f(sks), kb = lds_f(sks + 32), va = lds_f(sks + 64), vb = lds_f(sks + 96);
             const bool whole = pos0 + (int32_t)Q8_BS <= lim_min;   // every row sees the whole tile
-            // ---- exponent of the weights: follows the largest value scale that any row of the tile sees
-            float vtop = 0.0f;
+            float x[NQ][2], p[NQ][2], most = -INFINITY;   // q . k without scales; exponents 2^..; the largest of these
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int32_t pos = pos0 + (c >> 1) * 8 + 2 * (int32_t)t + (c & 1);
-                const float v = fabsf(vscale[c]);
-                if (pos < lim_max && v < INFINITY) vtop = fmaxf(vtop, v);
-            }
-            vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
-            vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
-            const int ve = (int)(__float_as_uint(vtop) >> 23) - 126;   // vtop < 2^ve
-            float regrade = 1.0f;
-            if (ve > v_exp) { regrade = ve - v_exp > 120 ? 0.0f : pow2i(v_exp - ve); v_exp = ve; }   // warp-uniform
-            const float vf = pow2i(13 - v_exp > 126 ? 126 : 13 - v_exp);
-            // ---- running maximum and sum, weights
-            uint32_t pw[4];   // A operand of P . V
-            float corr[NR];
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                float s[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const float dot = PIECES == 2 ? sc[c >> 1][c & 1] + sc[c >> 1][2 + (c & 1)] : sc[c >> 1][2 * r + (c & 1)];
-                    s[c] = dot * (row_scale[r] * kscale[c]);
+            for (int u = 0; u < NQ; u++) {
+                if constexpr (DIGITS == 3) {
+                    x[u][0] = fmaf((float)(dot[u][0][0] * 256 + dot[u][0][1]), 256.0f, (float)dot[u][1][0]);
+                    x[u][1] = fmaf((float)(dot[u][0][2] * 256 + dot[u][0][3]), 256.0f, (float)dot[u][1][2]);
+                } else {
+                    x[u][0] = (float)(dot[u][0][0] * 256 + dot[u][0][1]);
+                    x[u][1] = (float)(dot[u][0][2] * 256 + dot[u][0][3]);
                 }
-                if (!whole) {
+                // (a row without a reference yet has +infinity here for every score)
+                p[u][0] = fmaf(x[u][0], row_scale[u] * ka, -m_ref[u]);
+                p[u][1] = fmaf(x[u][1], row_scale[u] * kb, -m_ref[u]);
+                most = fmaxf(most, fmaxf(p[u][0], p[u][1]));
+            }
+            // A score more than 8 above its row's reference, or a value scale that the weights' power of two does not cover yet. (In a tile that not
+            // every row sees to its end, also by what nobody sees: the branch looks again.)
+            if (__any_sync(0xffffffffu, most > 8.0f || fmaxf(va, vb) >= pow2i(v_exp))) {
+                const int32_t pa = pos0 + (int32_t)g, pb = pa + 8;
+                float vtop = fmaxf(va < INFINITY && pa < lim_max ? va : 0.0f, vb < INFINITY && pb < lim_max ? vb : 0.0f);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const int32_t pos = pos0 + (c >> 1) * 8 + 2 * (int32_t)t + (c & 1);
-                        if (pos >= lim[r]) { s[c] = -INFINITY; }
+                for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
+                const int ve = (int)(__float_as_uint(vtop) >> 23) - 126;   // vtop < 2^ve
+                float regrade = 1.0f;
+                if (ve > v_exp) { regrade = ve - v_exp > 120 ? 0.0f : pow2i(v_exp - ve); v_exp = ve; }   // the same in every lane
+                float corr[NQ];
+#pragma unroll
+                for (int u = 0; u < NQ; u++) {
+                    const float s0 = x[u][0] * (row_scale[u] * ka), s1 = x[u][1] * (row_scale[u] * kb);
+                    float mb = fmaxf(pa < lim[u] ? s0 : -INFINITY, pb < lim[u] ? s1 : -INFINITY);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+                    const float m_new = fmaxf(m_ref[u], mb);
+                    corr[u] = m_new == -INFINITY ? 1.0f : ex2(m_ref[u] - m_new);
+                    m_ref[u] = m_new;
+                    p[u][0] = s0 - m_new;
+                    p[u][1] = s1 - m_new;
+                    l_run[u] *= corr[u];
+                    corr[u] *= regrade;
+                }
+#pragma unroll
+                for (int u = 0; u < NP; u++) {
+                    const float c0 = TWO ? corr[u] : corr[(2 * u) % NQ], c1 = TWO ? corr[u] : corr[(2 * u + 1) % NQ];
+#pragma unroll
+                    for (int j = 0; j < MT; j++) { acc[u][j][0] *= c0; acc[u][j][1] *= c1; acc[u][j][2] *= c0; acc[u][j][3] *= c1; }
+                }
+            }
+            const float vf = pow2i(5 - v_exp), fa = va * vf, fb = vb * vf;
+            float w[NQ][2];
+#pragma unroll
+            for (int u = 0; u < NQ; u++) {
+                p[u][0] = ex2(p[u][0]);
+                p[u][1] = ex2(p[u][1]);
+                w[u][0] = p[u][0] * fa;
+                w[u][1] = p[u][1] * fb;
+            }
+            if (!whole) {   // positions that a row does not see may hold anything, a NaN for a scale included
+                const int32_t pa = pos0 + (int32_t)g, pb = pa + 8;
+#pragma unroll
+                for (int u = 0; u < NQ; u++) {
+                    if (pa >= lim[u]) p[u][0] = w[u][0] = 0.0f;
+                    if (pb >= lim[u]) p[u][1] = w[u][1] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < NQ; u++) l_run[u] += p[u][0] + p[u][1];   // this lane's positions only: added up over the lanes at the end
+            uint32_t pw[NP][2];
+#pragma unroll
+            for (int u = 0; u < NP; u++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (TWO) {
+                        const float lead = __half2float(__float2half_rn(w[u][h]));
+                        pw[u][h] = transpose8(pack_half2(lead, w[u][h] - lead));
+                    } else {
+                        pw[u][h] = transpose8(pack_half2(w[(2 * u) % NQ][h], w[(2 * u + 1) % NQ][h]));
                     }
                 }
-                float mb = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-                mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
-                mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-                const float m_new = fmaxf(m_run[r], mb);
-                const float m_use = m_new == -INFINITY ? 0.0f : m_new;   // a row that has seen nothing yet
-                corr[r] = ex2(m_run[r] - m_use);
-                m_run[r] = m_new;
-                float wgt[4], sum = 0.0f;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const float p = ex2(s[c] - m_use);
-                    sum += p;
-                    const int32_t pos = pos0 + (c >> 1) * 8 + 2 * (int32_t)t + (c & 1);
-                    // positions a row does not see may hold anything, a NaN for a scale included
-                    wgt[c] = whole || pos < lim[r] ? p * (vscale[c] * vf) : 0.0f;
-                }
-                l_run[r] = l_run[r] * corr[r] + sum;   // this lane's positions only: the quad is added up at the end
-                const uint32_t h0 = pack_half2(wgt[0], wgt[1]), h1 = pack_half2(wgt[2], wgt[3]);
-                pw[r] = h0; pw[2 + r] = h1;
-                if constexpr (PIECES == 2) {
-                    const float2 b0 = unpack_half2(h0), b1 = unpack_half2(h1);
-                    pw[1] = pack_half2(wgt[0] - b0.x, wgt[1] - b0.y);
-                    pw[3] = pack_half2(wgt[2] - b1.x, wgt[3] - b1.y);
-                }
-            }
-            const float c0 = corr[0] * regrade, c1 = corr[NR - 1] * regrade;
-            if (__any_sync(0xffffffffu, c0 != 1.0f || c1 != 1.0f)) {
-#pragma unroll
-                for (int j = 0; j < NT; j++) { acc[j][0] *= c0; acc[j][1] *= c0; acc[j][2] *= c1; acc[j][3] *= c1; }
-            }
-            // ---- O += P . V
+            // ---- O^T += V p
             uint32_t w0[HD / 32], w1[HD / 32], w2[HD / 32], w3[HD / 32];
-            load_value<HD>(vsm, 2 * t, g, w0);
-            load_value<HD>(vsm, 2 * t + 1, g, w1);
-            load_value<HD>(vsm, 8 + 2 * t, g, w2);
-            load_value<HD>(vsm, 9 + 2 * t, g, w3);
+            at_lane.load_value(vsm + at_lane.val, w0);
+            at_lane.load_value(vsm + at_lane.val2, w1);
+            at_lane.load_value(vsm + at_lane.val + 8 * HD, w2);
+            at_lane.load_value(vsm + at_lane.val2 + 8 * HD, w3);
 #pragma unroll
-            for (int i4 = 0; i4 < HD / 32; i4++) {
-                const uint32_t a0 = w0[i4] ^ 0x80808080u, a1 = w1[i4] ^ 0x80808080u, a2 = w2[i4] ^ 0x80808080u, a3 = w3[i4] ^ 0x80808080u;
-                const uint32_t lo01 = __byte_perm(a0, a1, 0x5140), lo23 = __byte_perm(a0, a1, 0x7362);   // (d, d+1) and (d+2, d+3), position pairs
+            for (int j = 0; j < HD / 32; j++) {
+                const uint32_t a0 = w0[j] ^ 0x80808080u, a1 = w1[j] ^ 0x80808080u, a2 = w2[j] ^ 0x80808080u, a3 = w3[j] ^ 0x80808080u;
+                // bytes of two positions side by side: values 4j, 4j + 1 and 4j + 2, 4j + 3 of the lane's HD / 8
+                const uint32_t lo01 = __byte_perm(a0, a1, 0x5140), lo23 = __byte_perm(a0, a1, 0x7362);
                 const uint32_t hi01 = __byte_perm(a2, a3, 0x5140), hi23 = __byte_perm(a2, a3, 0x7362);
-                mma_f16(acc[4 * i4 + 0], pw[0], pw[1], pw[2], pw[3], half2_of(lo01, 0x4140), half2_of(hi01, 0x4140));
-                mma_f16(acc[4 * i4 + 1], pw[0], pw[1], pw[2], pw[3], half2_of(lo01, 0x4342), half2_of(hi01, 0x4342));
-                mma_f16(acc[4 * i4 + 2], pw[0], pw[1], pw[2], pw[3], half2_of(lo23, 0x4140), half2_of(hi23, 0x4140));
-                mma_f16(acc[4 * i4 + 3], pw[0], pw[1], pw[2], pw[3], half2_of(lo23, 0x4342), half2_of(hi23, 0x4342));
+                const uint32_t x0 = half2_of(lo01, 0x4140), x1 = half2_of(lo01, 0x4342), x2 = half2_of(hi01, 0x4140), x3 = half2_of(hi01, 0x4342);
+                const uint32_t y0 = half2_of(lo23, 0x4140), y1 = half2_of(lo23, 0x4342), y2 = half2_of(hi23, 0x4140), y3 = half2_of(hi23, 0x4342);
+#pragma unroll
+                for (int u = 0; u < NP; u++) {
+                    mma_f16(acc[u][2 * j], x0, x1, x2, x3, pw[u][0], pw[u][1]);
+                    mma_f16(acc[u][2 * j + 1], y0, y1, y2, y3, pw[u][0], pw[u][1]);
+                }
             }
         }
+        get = get == ring + (STAGES - 1) * C::STAGE ? ring : get + C::STAGE;
+        pos0 += (int32_t)(warps * Q8_BS);
         __syncwarp();
     }
     cp_wait<0>();
 
     // ---- the warps' results, in true units, over the ring: [warp][row][HD]
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
-        if (t == 0) { s_m[warp][g + 8 * r] = m_run[r]; s_l[warp][g + 8 * r] = l_run[r]; }
+    for (int u = 0; u < NQ; u++) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l_run[u] += __shfl_xor_sync(0xffffffffu, l_run[u], o);
+        if (g == 0) { s_m[warp][4 * u + t] = m_ref[u]; s_l[warp][4 * u + t] = l_run[u]; }
     }
     __syncthreads();   // every warp is done with its ring
     float* part = reinterpret_cast<float*>(smem);
     {
-        const float un = pow2i(v_exp - 13 < -126 ? -126 : v_exp - 13);
-        float* wp = part + (size_t)warp * ROWS * HD;
-        // accumulator columns 2t, 2t + 1 of tile j are n = 2t, 2t + 1: values HD / 8 * n + j
+        const float un = pow2i(v_exp - 5);
+        float* wp = part + (size_t)warp * ROWS * HD + (HD / 8) * g;
+        // rows g and g + 8 of tile j are values 2j and 2j + 1 of the lane's HD / 8, columns 2t and 2t + 1 the parts of a query or two queries
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
+        for (int u = 0; u < NP; u++)
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const uint32_t d = (HD / 8) * (2 * t + c) + j;
-                if (PIECES == 2) wp[g * HD + d] = (acc[j][c] + acc[j][2 + c]) * un;
-                else {
-                    wp[g * HD + d] = acc[j][c] * un;
-                    wp[(g + 8) * HD + d] = acc[j][2 + c] * un;
+            for (int j = 0; j < MT; j++) {
+                if constexpr (TWO) {
+                    *reinterpret_cast<float2*>(wp + (4 * u + t) * HD + 2 * j) =
+                        make_float2((acc[u][j][0] + acc[u][j][1]) * un, (acc[u][j][2] + acc[u][j][3]) * un);
+                } else {
+                    *reinterpret_cast<float2*>(wp + (8 * u + t) * HD + 2 * j) = make_float2(acc[u][j][0] * un, acc[u][j][2] * un);
+                    *reinterpret_cast<float2*>(wp + (8 * u + 4 + t) * HD + 2 * j) = make_float2(acc[u][j][1] * un, acc[u][j][3] * un);
                 }
+            }
+    }
+    __syncthreads();
+    if (n_splits > 1) cluster_wait_all();
+    // ---- merged over the warps, and stored or (with splits) put in place of warp 0's
+    if (threadIdx.x < ROWS) {
+        const uint32_t r = threadIdx.x;
+        float M = s_m[0][r], L = 0.0f;
+        for (uint32_t w = 1; w < warps; w++) M = fmaxf(M, s_m[w][r]);
+        const float use = M == -INFINITY ? 0.0f : M;
+        for (uint32_t w = 0; w < warps; w++) L += s_l[w][r] * ex2(s_m[w][r] - use);
+        const float norm = n_splits > 1 ? 1.0f : (L == 0.0f ? 0.0f : 1.0f / L);   // a row that sees nothing is zero
+        for (uint32_t w = 0; w < warps; w++) s_f[w][r] = ex2(s_m[w][r] - use) * norm;
+        if (n_splits > 1) {   // to every CTA of the cluster (which all run by now: see the arrival above)
+            cg::cluster_group cluster = cg::this_cluster();
+            for (uint32_t k = 0; k < n_splits; k++) {
+                *cluster.map_shared_rank(&s_top[split][r], k) = M;
+                *cluster.map_shared_rank(&s_sum[split][r], k) = L;
             }
         }
     }
     __syncthreads();
-    // ---- merged over the warps into [row][HD] (in place of warp 0's)
-    for (uint32_t i = threadIdx.x; i < (last + 1) * HD; i += AQ_WARPS * 32) {
-        const uint32_t r = i / HD;
-        float M = s_m[0][r];
-#pragma unroll
-        for (int w = 1; w < AQ_WARPS; w++) M = fmaxf(M, s_m[w][r]);
-        const float use = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f, o = 0.0f;
-#pragma unroll
-        for (int w = 0; w < AQ_WARPS; w++) {
-            const float f = ex2(s_m[w][r] - use);
-            L += s_l[w][r] * f;
-            o += part[w * ROWS * HD + i] * f;
-        }
-        part[i] = o;
-        if (i % HD == 0) { s_top[r] = M; s_sum[r] = L; }
-    }
     T* out = reinterpret_cast<T*>(a.out);
-    if (n_splits == 1) {
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < (last + 1) * HD; i += AQ_WARPS * 32) {
-            const uint32_t r = i / HD;
-            const float L = s_sum[r];
-            out[q_index(r) + i % HD] = Cvt<T>::from_f(L == 0.0f ? 0.0f : part[i] / L);   // a row that sees nothing is zero
+    auto store = [&](uint32_t r, uint32_t d, float4 o) {
+        T* dst = out + s_at[r] + d;
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(dst) = o;
+        } else {
+            const bf162 x = __floats2bfloat162_rn(o.x, o.y), y = __floats2bfloat162_rn(o.z, o.w);
+            *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
         }
-        return;
+    };
+    for (uint32_t i = threadIdx.x; i < (last + 1) * (HD / 4); i += blockDim.x) {
+        const uint32_t r = i / (HD / 4);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t w = 0; w < warps; w++) {
+            const float4 v = *reinterpret_cast<const float4*>(part + w * ROWS * HD + 4 * i);
+            const float f = s_f[w][r];
+            o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+        }
+        if (n_splits == 1) store(r, 4 * i % HD, o);
+        else *reinterpret_cast<float4*>(part + 4 * i) = o;
     }
+    if (n_splits == 1) return;
     // ---- and over the splits: every CTA of the cluster finishes its share of the values
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    for (uint32_t i = split * (AQ_WARPS * 32) + threadIdx.x; i < (last + 1) * HD; i += n_splits * AQ_WARPS * 32) {
-        const uint32_t r = i / HD;
-        float M = -INFINITY;
-        for (uint32_t s = 0; s < n_splits; s++) M = fmaxf(M, *cluster.map_shared_rank(&s_top[r], s));
+    if (threadIdx.x < ROWS) {
+        const uint32_t r = threadIdx.x;
+        float M = -INFINITY, L = 0.0f;
+        for (uint32_t k = 0; k < n_splits; k++) M = fmaxf(M, s_top[k][r]);
         const float use = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f, o = 0.0f;
-        for (uint32_t s = 0; s < n_splits; s++) {
-            const float f = ex2(*cluster.map_shared_rank(&s_top[r], s) - use);
-            L += *cluster.map_shared_rank(&s_sum[r], s) * f;
-            o += *cluster.map_shared_rank(&part[i], s) * f;
+        for (uint32_t k = 0; k < n_splits; k++) {
+            s_f[k][r] = ex2(s_top[k][r] - use);
+            L += s_sum[k][r] * s_f[k][r];
         }
-        out[q_index(r) + i % HD] = Cvt<T>::from_f(L == 0.0f ? 0.0f : o / L);
+        s_l[0][r] = L == 0.0f ? 0.0f : 1.0f / L;
+    }
+    __syncthreads();
+    for (uint32_t i = split * blockDim.x + threadIdx.x; i < (last + 1) * (HD / 4); i += n_splits * blockDim.x) {
+        const uint32_t r = i / (HD / 4);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (uint32_t k = 0; k < n_splits; k++) {
+            const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + 4 * i, k));
+            const float f = s_f[k][r];
+            o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+        }
+        const float norm = s_l[0][r];
+        store(r, 4 * i % HD, make_float4(o.x * norm, o.y * norm, o.z * norm, o.w * norm));
     }
     cluster.sync();   // nobody leaves while a peer may still read its results
 }
 
-// Splits: as many CTAs as two for every SM, but no fewer than 8 blocks (two a warp) each.
-static uint32_t aq_pick_splits(uint64_t units, uint32_t max_blocks) {
-    uint32_t s = 1;
-    while (s < AQ_MAX_SPLITS && units * s * 2 <= 2 * B200_SMS && max_blocks / (2 * s) >= 8) s *= 2;
-    return s;
+// Warps of a CTA and splits of a sequence, for `room` warps on all SMs together.
+// 8 warps instead of 4 where the sequences are long (128 blocks and more: the CTAs' starts and ends weigh less; 64 x 16 heads x 128 up to
+// 4096 positions 90 against 95 us, but 64 x 12 heads x 64 up to 512 16.4 against 13.0) or where all of them fit at once (8 x 12 heads 6.0 against
+// 6.6 us).
+// Split while that leaves 16 tiles to a warp and every CTA finds room at once (8 kv heads x 2 tiles of queries x 2 sequences of 60000: 93 us in 4, 63 in
+// 8, 90 in 16). Halves may take two waves (32 x 8 heads up to 8192: 58 us whole, 53 halved, 59 in quarters: ragged sequences end at different
+// times, and an exchange costs about a microsecond, hidden only behind other CTAs' streams).
+static void aq_plan(uint64_t units, uint32_t max_blocks, uint32_t room, uint32_t& warps, uint32_t& n_splits) {
+    warps = max_blocks >= 128 || units * 8 <= room ? 8 : 4;
+    if (n_splits) return;
+    n_splits = 1;
+    while (n_splits < AQ_MAX_SPLITS && units * warps * (n_splits == 1 ? 1 : 2 * n_splits) <= room && max_blocks / (2 * n_splits * warps) >= 16) n_splits *= 2;
 }
 
-template <typename T, int HD, int PIECES>
+template <typename T, int HD, int NQ, bool TWO>
 static int aq_launch(cudaStream_t st, AqArgs a, uint32_t rows, uint32_t n_splits) {
-    constexpr uint32_t ROWS = PIECES == 2 ? 8 : 16;
+    constexpr uint32_t ROWS = 4 * NQ;
     using C = AqCfg<HD>;
-    constexpr size_t merge = (size_t)AQ_WARPS * ROWS * HD * 4;
-    constexpr size_t smem = merge > (size_t)C::RING ? merge : (size_t)C::RING;
+    constexpr size_t merge = (size_t)ROWS * HD * 4, ring = (size_t)C::STAGES * C::STAGE, per_warp = merge > ring ? merge : ring;
     a.q_tiles = cdiv(a.q_len * a.group, ROWS);
     const uint64_t units = (uint64_t)rows * a.kv_heads * a.q_tiles;
     AK_REQUIRE(units <= 0x7fffffffu, AK_ERR_UNSUPPORTED, "ak_attn_decode_paged_q8: %u rows x %u heads x %u tiles of queries are too many for one call", rows,
                a.kv_heads, a.q_tiles);
-    if (!n_splits) n_splits = aq_pick_splits(units, a.max_blocks);
+    uint32_t warps;
     while (n_splits & (n_splits - 1)) n_splits &= n_splits - 1;   // a cluster of a power of two of CTAs
+    aq_plan(units, a.max_blocks, C::CTAS * AQ_MAX_WARPS * B200_SMS, warps, n_splits);
     {
         static bool attr_set[64] = {};
         int dev = 0;
         AK_CUDA(cudaGetDevice(&dev));
         std::lock_guard<std::mutex> lock(device_cache_mutex());
         if (!attr_set[dev & 63]) {
-            AK_CUDA(cudaFuncSetAttribute(attn_decode_q8_kernel<T, HD, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            AK_CUDA(cudaFuncSetAttribute(attn_decode_q8_kernel<T, HD, PIECES>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            AK_CUDA(cudaFuncSetAttribute(attn_decode_q8_kernel<T, HD, NQ, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(per_warp * AQ_MAX_WARPS)));
+            AK_CUDA(cudaFuncSetAttribute(attn_decode_q8_kernel<T, HD, NQ, TWO>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
             attr_set[dev & 63] = true;
         }
     }
-    return launch_k(attn_decode_q8_kernel<T, HD, PIECES>, dim3((unsigned)units, 1, n_splits), dim3(AQ_WARPS * 32), smem, st,
+    return launch_k(attn_decode_q8_kernel<T, HD, NQ, TWO>, dim3((unsigned)units, 1, n_splits), dim3(warps * 32), per_warp * warps, st,
                     n_splits > 1 ? dim3(1, 1, n_splits) : NO_CLUSTER, a);
+}
+
+// The query rows of a kv head choose the form: f32, and up to 4 rows, go 4 to a CTA with weights in two parts, bf16 with more rows 8 to a CTA with the
+// leading part. Further tiles of queries read the cache again, from L2 mostly: 16 rows as one tile (168 registers, 12 warps on an SM)
+// took 71 us where two tiles of 8 take 63 (2 sequences of 60000, 8 kv heads x 128).
+template <int HD>
+static int aq_form(cudaStream_t st, const AqArgs& a, const ak_attn_q8_params& p) {
+    if (p.dtype == AK_F32) return aq_launch<float, HD, 1, true>(st, a, p.rows, p.n_splits);
+    if ((uint64_t)a.q_len * a.group <= 4) return aq_launch<bf16, HD, 1, true>(st, a, p.rows, p.n_splits);
+    return aq_launch<bf16, HD, 2, false>(st, a, p.rows, p.n_splits);
 }
 
 }  // namespace ak
@@ -510,16 +654,10 @@ extern "C" int ak_attn_decode_paged_q8(void* stream, const void* q, const int8_t
     const uint32_t group = p.heads / p.kv_heads;
     const AqArgs a{q, k_pool, v_pool, k_scales, v_scales, block_tables, kv_lens, out, p.q_len, p.heads, p.kv_heads, group, 1, p.max_blocks_per_seq,
                    p.pool_blocks, p.scale};
-    const bool two = p.dtype == AK_F32 || (uint64_t)p.q_len * group <= 8;
-#define AK_ATTN_Q8(HD)                                                                                         \
-    return p.dtype == AK_F32 ? aq_launch<float, HD, 2>(as_stream(stream), a, p.rows, p.n_splits)              \
-           : two             ? aq_launch<bf16, HD, 2>(as_stream(stream), a, p.rows, p.n_splits)               \
-                             : aq_launch<bf16, HD, 1>(as_stream(stream), a, p.rows, p.n_splits)
     switch (p.head_dim) {
-        case 32: AK_ATTN_Q8(32);
-        case 64: AK_ATTN_Q8(64);
-        case 96: AK_ATTN_Q8(96);
-        default: AK_ATTN_Q8(128);
+        case 32: return aq_form<32>(as_stream(stream), a, p);
+        case 64: return aq_form<64>(as_stream(stream), a, p);
+        case 96: return aq_form<96>(as_stream(stream), a, p);
+        default: return aq_form<128>(as_stream(stream), a, p);
     }
-#undef AK_ATTN_Q8
 }

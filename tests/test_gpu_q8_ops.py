@@ -317,7 +317,7 @@ def _attn_check(torch, out, q, cache, tables, lens, q_len, heads, kv_heads, hd, 
     kp, vp, ks, vs = (t.double() for t in cache)
     group = heads // kv_heads
     out, q = out.double().view(len(lens), q_len, kv_heads, group, hd), q.double().view(len(lens), q_len, kv_heads, group, hd)
-    rounded = dtype == "bf16" and q_len * group > 8      # weights rounded to f16
+    rounded = dtype == "bf16" and q_len * group > 4      # weights rounded to f16
     for r, n in enumerate(lens):
         ids = tables[r].long()
         pos = torch.arange(min(max(n, 0), tables.shape[1] * 16), device="cuda")
@@ -334,9 +334,12 @@ def _attn_check(torch, out, q, cache, tables, lens, q_len, heads, kv_heads, hd, 
             size = torch.einsum("kgd,jkd->kgj", q[r, i].abs(), k.abs()) * abs(scale)
             w = torch.softmax(s, -1)
             want, mass = torch.einsum("kgj,jkd->kgd", w, v), torch.einsum("kgj,jkd->kgd", w, v.abs())
-            # A score: queries in 22 bits, HD / 16 steps of the tensor core and the scales, each off by at most 2^-22 of the terms. A weight: that
+            # A score: HD / 16 steps of a sum and the scales, each off by at most 2^-22 of the terms, and what the query is off. A weight: that
             # (and the maximum's, alike), exp2 and the exponent's rounding. The sums: a step of the tensor core per 16 positions.
-            ds = float(size.max()) * (hd / 16 + 6) * 2.0 ** -22
+            # Queries are integers of D base-256 digits, half a step of 127 * 256^(D - 1) of the head's largest value.
+            digits = q[r, i].abs().amax(-1, keepdim=True) * 2.0 ** (-24 if dtype == "f32" else -16)
+            size = size * (hd / 16 + 6) * 2.0 ** -22 + torch.einsum("kgd,jkd->kgj", digits.expand(q[r, i].shape), k.abs()) * abs(scale)
+            ds = float(size.max())
             rel = 2 * (ds + 2.0 ** -21) + (len(p) / 16 + 40) * 2.0 ** -22 + (2.0 ** -11 if rounded else 0)
             tol = rel * mass + HALF[dtype] * want.abs()
             err = (out[r, i] - want).abs()
