@@ -19,97 +19,98 @@ int q8_check_here(const void* p, const char* who) {
 // ============================================================================ norm + quantisation
 // h = x (+ residual, written back), y = h / sqrt(mean(h^2) + eps) * w (w == nullptr: y = h), q = rint(127 y / max|y|), s = max|y| / 127.
 // One pass: a row lives in the registers of its threads between the two reductions (sum of squares, largest magnitude), so that every
-// input byte is read once and every output byte written once. `tpr` threads share a row, each holding NV groups of 4 consecutive values.
+// input byte is read once and every output byte written once. `tpr` threads share a row.
 //
-// RAG: size % 4 != 0. All the arrays of a row start at the same element offset, so groups are cut where the ADDRESS is a multiple of 4
-// elements: the first and last group of a row are partial (element by element), all others are whole vectors.
-template <typename T> struct Q8Vec;
-template <> struct Q8Vec<float> {
-    static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-        const float4 t = *reinterpret_cast<const float4*>(p);
-        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-    }
-};
-template <> struct Q8Vec<bf16> {
-    static __device__ __forceinline__ void load(const bf16* p, float (&v)[4]) {
-        const uint2 t = *reinterpret_cast<const uint2*>(p);
-        v[0] = __uint_as_float(t.x << 16); v[1] = __uint_as_float(t.x & 0xffff0000u);
-        v[2] = __uint_as_float(t.y << 16); v[3] = __uint_as_float(t.y & 0xffff0000u);
+// What bounds it once the bytes do not: instructions, some 200 of them per warp and row for the reductions and scales (IEEE divisions and roots
+// made that 300), so long rows take several values a thread and rows of up to 1024 values one warp.
+template <typename T> struct Q8Vec {
+    static constexpr int V = 16 / sizeof(T);   // values of a group: a 16-byte load
+    static __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
+        const uint4 t = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            if constexpr (sizeof(T) == 4) v[e] = __uint_as_float(w[e]);
+            else v[e] = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        }
     }
 };
 
 constexpr uint32_t NQ_MAX_WARPS = 32;
 
-template <typename T, bool RAG, int NV>
+// The sum of a row's threads' values, in the same order in every thread; the largest of their (unsigned) values.
+__device__ __forceinline__ float row_sum(float v, float* s_sum, uint32_t warps, uint32_t wid, uint32_t lane) {
+    v = warp_sum(v);
+    if (warps == 1) return v;
+    if (lane == 0) s_sum[wid] = v;
+    __syncthreads();
+    v = 0.0f;
+    for (uint32_t i = 0; i < warps; i++) v += s_sum[i];
+    return v;
+}
+__device__ __forceinline__ uint32_t row_top(uint32_t v, uint32_t* s_top, uint32_t warps, uint32_t wid, uint32_t lane) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (warps == 1) return v;
+    if (lane == 0) s_top[wid] = v;
+    __syncthreads();
+    return __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
+}
+
+// Rows of whole vectors: a thread holds NV groups of V consecutive values (16 bytes of input).
+template <typename T, int NV>
 __global__ void __launch_bounds__(1024)
 norm_q8_kernel(T* __restrict__ x, const float* __restrict__ residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales,
-               uint32_t rows, uint32_t size, float eps, uint32_t w_vec) {
+               uint32_t rows, uint32_t size, float eps) {
+    constexpr int V = Q8Vec<T>::V;
     pdl_wait();
     pdl_trigger();
     __shared__ float s_sum[NQ_MAX_WARPS];
     __shared__ uint32_t s_top[NQ_MAX_WARPS];
-    const uint32_t tpr = blockDim.x, t = threadIdx.x, lane = t & 31, wid = t >> 5, warps = tpr >> 5;
+    const uint32_t tpr = blockDim.x, t = threadIdx.x, lane = t & 31, wid = t >> 5, warps = tpr >> 5, groups = size / V;
     const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;   // blockDim.y > 1 only with one warp per row
     if (row >= rows) return;
-    const size_t off = (size_t)row * size;
-    const uint32_t shift = RAG ? (uint32_t)(off & 3) : 0;
-    const uint32_t groups = (shift + size + 3) >> 2;
-    float v[NV][4];
-    float ss = 0.0f;
+    x += (size_t)row * size;
+    q += (size_t)row * size;
+    float y[NV][V];
 #pragma unroll
     for (int c = 0; c < NV; c++) {
         const uint32_t g = t + c * tpr;
-        v[c][0] = v[c][1] = v[c][2] = v[c][3] = 0.0f;
-        if (g >= groups) continue;
-        const int32_t e0 = (int32_t)(4 * g - shift);
-        if (!RAG || (e0 >= 0 && (uint32_t)e0 + 4 <= size)) {
-            T* xp = x + off + e0;
-            Q8Vec<T>::load(xp, v[c]);
-            if constexpr (sizeof(T) == 4) {
-                if (residual) {
-                    float r[4];
-                    Q8Vec<float>::load(residual + off + e0, r);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[c][e] += r[e];
-                    *reinterpret_cast<float4*>(xp) = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
-                }
-            }
-        } else {
+        for (int e = 0; e < V; e++) y[c][e] = 0.0f;
+        if (g < groups) Q8Vec<T>::load(x + V * g, y[c]);
+    }
+    if constexpr (sizeof(T) == 4) {
+        if (residual) {
+            residual += (size_t)row * size;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int32_t i = e0 + e;
-                if (i < 0 || (uint32_t)i >= size) continue;
-                v[c][e] = Cvt<T>::to_f(x[off + i]);
-                if constexpr (sizeof(T) == 4) {
-                    if (residual) { v[c][e] += residual[off + i]; x[off + i] = v[c][e]; }
-                }
+            for (int c = 0; c < NV; c++) {
+                const uint32_t g = t + c * tpr;
+                if (g >= groups) continue;
+                float r[4];
+                Q8Vec<float>::load(residual + V * g, r);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[c][e] += r[e];
+                *reinterpret_cast<float4*>(x + V * g) = make_float4(y[c][0], y[c][1], y[c][2], y[c][3]);
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; e++) ss += v[c][e] * v[c][e];
     }
     if (w) {
-        ss = warp_sum(ss);
-        if (warps > 1) {
-            if (lane == 0) s_sum[wid] = ss;
-            __syncthreads();
-            ss = warp_sum(lane < warps ? s_sum[lane] : 0.0f);   // the same order in every warp
-        }
-        const float rs = 1.0f / sqrtf(ss / (float)size + eps);
+        float ss = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NV; c++)
+#pragma unroll
+            for (int e = 0; e < V; e++) ss += y[c][e] * y[c][e];
+        const float rs = rsqrtf(row_sum(ss, s_sum, warps, wid, lane) / (float)size + eps);
 #pragma unroll
         for (int c = 0; c < NV; c++) {
             const uint32_t g = t + c * tpr;
             if (g >= groups) continue;
-            const int32_t e0 = (int32_t)(4 * g - shift);
-            if (w_vec && (!RAG || (shift == 0 && (uint32_t)e0 + 4 <= size))) {
+#pragma unroll
+            for (int k = 0; k < V; k += 4) {
                 float ww[4];
-                Q8Vec<float>::load(w + e0, ww);
+                Q8Vec<float>::load(w + V * g + k, ww);
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[c][e] = v[c][e] * rs * ww[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (e0 + e >= 0 && (uint32_t)(e0 + e) < size) v[c][e] = v[c][e] * rs * w[e0 + e];
+                for (int e = 0; e < 4; e++) y[c][k + e] = y[c][k + e] * rs * ww[e];
             }
         }
     }
@@ -117,33 +118,150 @@ norm_q8_kernel(T* __restrict__ x, const float* __restrict__ residual, const floa
 #pragma unroll
     for (int c = 0; c < NV; c++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = max(top, abs_bits(v[c][e]));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (warps > 1) {
-        if (lane == 0) s_top[wid] = top;
-        __syncthreads();
-        top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
-    }
+        for (int e = 0; e < V; e++) top = max(top, abs_bits(y[c][e]));
     float inv, s;
-    q8_scale(top, inv, s);
+    q8_scale(row_top(top, s_top, warps, wid, lane), inv, s);
+    const bool ok = s == s;
     if (t == 0) scales[row] = s;
 #pragma unroll
     for (int c = 0; c < NV; c++) {
         const uint32_t g = t + c * tpr;
         if (g >= groups) continue;
-        const int32_t e0 = (int32_t)(4 * g - shift);
-        if (!RAG || (e0 >= 0 && (uint32_t)e0 + 4 <= size)) {
-            *reinterpret_cast<uint32_t*>(q + off + e0) = q8_pack4(v[c][0], v[c][1], v[c][2], v[c][3], inv);
-        } else {
+        uint32_t o[V / 4];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (e0 + e >= 0 && (uint32_t)(e0 + e) < size) q[off + e0 + e] = (int8_t)q8_of(v[c][e], inv);
-        }
+        for (int k = 0; k < V / 4; k++) o[k] = q8_pack4(y[c][4 * k], y[c][4 * k + 1], y[c][4 * k + 2], y[c][4 * k + 3], inv, ok);
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(q + V * g) = make_uint2(o[0], o[1]);
+        else *reinterpret_cast<uint32_t*>(q + V * g) = o[0];
     }
 }
 
-// Rows that do not fit the registers of a block (over 32768 values), and buffers that are not aligned for vectors: a block per row, three
-// passes over it (the second and third read what the first wrote back). y is computed twice by the same operations, hence with the same bits.
+// Rows of any size. All the arrays of a row start at the same element offset, so groups are cut where the ADDRESS is a multiple of V elements; the
+// first and last group of a row are partial. With weights (KEEP), resident blocks walk over the rows with a stride that is a multiple of V, so that a block
+// sees one shift only: which of a thread's groups are partial and its weights (in registers) are settled once: 16384 x 2047 45 us, where a
+// block per row, its weights put together from two neighbouring vectors, took 56. Without weights there is nothing to keep, and with a
+// residual the loads want blocks coming and going.
+template <typename T, int NV, bool KEEP>
+__global__ void __launch_bounds__(KEEP ? 512 : 1024, KEEP ? 2 : 1)
+norm_q8_ragged_kernel(T* __restrict__ x, const float* __restrict__ residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales,
+                      uint32_t rows, uint32_t size, float eps) {
+    constexpr int V = Q8Vec<T>::V;
+    pdl_wait();
+    pdl_trigger();
+    __shared__ float s_sum[NQ_MAX_WARPS];
+    __shared__ uint32_t s_top[2][NQ_MAX_WARPS];
+    const uint32_t tpr = blockDim.x, t = threadIdx.x, lane = t & 31, wid = t >> 5, warps = tpr >> 5;
+    uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;   // blockDim.y > 1 only with one warp per row
+    if (row >= rows) return;
+    const uint32_t step = gridDim.x * blockDim.y;           // a multiple of V, or there is no second row
+    const uint32_t shift = (uint32_t)(((size_t)row * size) & (V - 1)), groups = (shift + size + V - 1) / V;
+    auto inside = [&](int32_t i) { return i >= 0 && (uint32_t)i < size; };
+    float ww[KEEP ? NV : 1][V];
+    bool some[NV], part[NV];
+#pragma unroll
+    for (int c = 0; c < NV; c++) {
+        const int32_t e0 = (int32_t)(V * (t + c * tpr) - shift);
+        some[c] = t + c * tpr < groups;
+        part[c] = some[c] && !(e0 >= 0 && (uint32_t)e0 + V <= size);
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int e = 0; e < V; e++) ww[c][e] = inside(e0 + e) ? w[e0 + e] : 0.0f;
+        }
+    }
+    for (uint32_t turn = 0; row < rows; row += step, turn ^= 1) {
+        const size_t off = (size_t)row * size - shift;   // of group 0 (which may begin in the row before)
+        T* xr = x + off;
+        int8_t* qr = q + off;
+        float y[NV][V];
+#pragma unroll
+        for (int c = 0; c < NV; c++) {
+            const uint32_t at = V * (t + c * tpr);
+#pragma unroll
+            for (int e = 0; e < V; e++) y[c][e] = 0.0f;
+            if (!some[c]) continue;
+            // a partial group is read whole too, with values of the neighbouring rows that are dropped, but for one that would reach past the last row
+            if (!part[c] || row + 1 < rows || at + V <= shift + size) Q8Vec<T>::load(xr + at, y[c]);
+            else {
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (at + e >= shift && at + e < shift + size) y[c][e] = Cvt<T>::to_f(xr[at + e]);
+            }
+        }
+        if constexpr (sizeof(T) == 4) {
+            if (residual) {
+                const float* rr = residual + off;
+#pragma unroll
+                for (int c = 0; c < NV; c++) {
+                    const uint32_t at = V * (t + c * tpr);
+                    if (!some[c]) continue;
+                    if (!part[c]) {
+                        float r[4];
+                        Q8Vec<float>::load(rr + at, r);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[c][e] += r[e];
+                        *reinterpret_cast<float4*>(xr + at) = make_float4(y[c][0], y[c][1], y[c][2], y[c][3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; e++)
+                            if (at + e >= shift && at + e < shift + size) { y[c][e] += rr[at + e]; xr[at + e] = y[c][e]; }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NV; c++)
+            if (part[c]) {
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (!inside((int32_t)(V * (t + c * tpr) - shift) + e)) y[c][e] = 0.0f;
+            }
+        if (w) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NV; c++)
+#pragma unroll
+                for (int e = 0; e < V; e++) ss += y[c][e] * y[c][e];
+            const float rs = rsqrtf(row_sum(ss, s_sum, warps, wid, lane) / (float)size + eps);
+#pragma unroll
+            for (int c = 0; c < NV; c++) {
+                const int32_t e0 = (int32_t)(V * (t + c * tpr) - shift);
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    if constexpr (KEEP) y[c][e] = y[c][e] * rs * ww[c][e];
+                    else if (inside(e0 + e)) y[c][e] = y[c][e] * rs * w[e0 + e];
+                }
+            }
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < NV; c++)
+#pragma unroll
+            for (int e = 0; e < V; e++) top = max(top, abs_bits(y[c][e]));
+        float inv, s;
+        q8_scale(row_top(top, s_top[turn], warps, wid, lane), inv, s);   // two buffers: a warp may be a row ahead of another that still reads
+        const bool ok = s == s;
+        if (t == 0) scales[row] = s;
+#pragma unroll
+        for (int c = 0; c < NV; c++) {
+            const uint32_t at = V * (t + c * tpr);
+            if (!some[c]) continue;
+            uint32_t o[V / 4];
+#pragma unroll
+            for (int k = 0; k < V / 4; k++) o[k] = q8_pack4(y[c][4 * k], y[c][4 * k + 1], y[c][4 * k + 2], y[c][4 * k + 3], inv, ok);
+            if (!part[c]) {
+                if constexpr (V == 8) *reinterpret_cast<uint2*>(qr + at) = make_uint2(o[0], o[1]);
+                else *reinterpret_cast<uint32_t*>(qr + at) = o[0];
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (at + e >= shift && at + e < shift + size) qr[at + e] = (int8_t)(o[e / 4] >> (8 * (e % 4)));
+            }
+        }
+        if (!KEEP) break;
+    }
+}
+
+// Rows that do not fit the registers of a block, and buffers that are not aligned for vectors: a block per row, three passes over it (the second and third read what the first wrote back). y is
+// computed twice by the same operations, hence with the same bits.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 norm_q8_any_kernel(T* x, const float* residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales, uint32_t size, float eps) {
@@ -167,7 +285,7 @@ norm_q8_any_kernel(T* x, const float* residual, const float* __restrict__ w, int
         if (lane == 0) s_sum[wid] = ss;
         __syncthreads();
         ss = warp_sum(lane < warps ? s_sum[lane] : 0.0f);
-        rs = 1.0f / sqrtf(ss / (float)size + eps);
+        rs = rsqrtf(ss / (float)size + eps);
     }
     auto value = [&](uint32_t i) { return w ? Cvt<T>::to_f(x[off + i]) * rs * w[i] : Cvt<T>::to_f(x[off + i]); };   // written by this thread
     uint32_t top = 0;
@@ -178,145 +296,229 @@ norm_q8_any_kernel(T* x, const float* residual, const float* __restrict__ w, int
     top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
     float inv, s;
     q8_scale(top, inv, s);
+    const bool ok = s == s;
     if (threadIdx.x == 0) scales[blockIdx.x] = s;
-    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x) q[off + i] = (int8_t)q8_of(value(i), inv);
-}
-
-template <typename T, bool RAG, int NV>
-static int norm_q8_launch(cudaStream_t st, T* x, const float* residual, const float* w, int8_t* q, float* scales, uint32_t rows, uint32_t size, float eps,
-                          uint32_t tpr) {
-    const uint32_t rpb = tpr == 32 ? 4 : 1;
-    return launch_k(norm_q8_kernel<T, RAG, NV>, dim3(cdiv(rows, rpb)), dim3(tpr, rpb), 0, st, NO_CLUSTER, x, residual, w, q, scales, rows, size, eps,
-                    (uint32_t)q8_aligned(w, 16));
+    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x) q[off + i] = q8_of(value(i), inv, ok);
 }
 
 template <typename T>
 static int norm_q8(cudaStream_t st, T* x, const float* residual, const float* w, int8_t* q, float* scales, uint32_t rows, uint32_t size, float eps) {
-    const uint32_t groups = (size + 3) / 4 + (size % 4 ? 1 : 0);   // of a row, at most
-    if (groups > 8192 || !q8_aligned(x, 4 * sizeof(T)) || !q8_aligned(residual, 16) || !q8_aligned(q, 4))
+    constexpr uint32_t V = Q8Vec<T>::V, MOST = 32 / V;   // 32 values a thread
+    const uint32_t groups = cdiv(size, V) + (size % V ? 1 : 0);   // of a row, at most
+    const bool vectors = q8_aligned(x, 16) && q8_aligned(residual, 16) && q8_aligned(q, V) && q8_aligned(w, 16);
+    if (!vectors || groups > 1024 * (size % V ? MOST / 2 : MOST))
         return launch_k(norm_q8_any_kernel<T>, dim3(rows), dim3(512), 0, st, NO_CLUSTER, x, residual, w, q, scales, size, eps);
-    uint32_t nv = 1;
-    if (rows > 2 * B200_SMS) nv = groups <= 64 ? 2 : (groups <= 1024 ? 4 : 8);
-    while (groups > nv * 1024) nv *= 2;
-    const uint32_t tpr = cdiv(groups, nv * 32) * 32;
-#define AK_NORM_Q8(NV)                                                                                     \
-    return size % 4 ? norm_q8_launch<T, true, NV>(st, x, residual, w, q, scales, rows, size, eps, tpr)    \
-                    : norm_q8_launch<T, false, NV>(st, x, residual, w, q, scales, rows, size, eps, tpr)
-    switch (nv) {
-        case 1: AK_NORM_Q8(1);
-        case 2: AK_NORM_Q8(2);
-        case 4: AK_NORM_Q8(4);
-        default: AK_NORM_Q8(8);
+    const bool few = rows <= 2 * B200_SMS;   // latency: as many threads to a row as there are vectors
+    if (size % V) {
+        uint32_t n = few ? 1 : groups <= 32 * MOST / 2 ? cdiv(groups, 32) : MOST / 2;   // 16 values a thread
+        if (n == 3) n = 4;
+        while (groups > n * 1024) n *= 2;
+        const uint32_t tpr = cdiv(groups, n * 32) * 32;
+        const dim3 block(tpr, tpr == 32 && !few ? 4 : 1);
+        const bool keep = w && !residual && !few && tpr <= 512;
+#define AK_NORM_Q8(N)                                                                                                                                         \
+    case N: {                                                                                                                                                 \
+        const uint32_t blocks = cdiv(rows, block.y);                                                                                                          \
+        if (!keep) return launch_k(norm_q8_ragged_kernel<T, N, false>, dim3(blocks), block, 0, st, NO_CLUSTER, x, residual, w, q, scales, rows, size, eps);   \
+        int occ = 0;                                                                                                                                          \
+        AK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, norm_q8_ragged_kernel<T, N, true>, (int)(block.x * block.y), 0));                         \
+        const uint32_t most = B200_SMS * (uint32_t)(occ < 1 ? 1 : occ) / V * V;                                                                               \
+        return launch_k(norm_q8_ragged_kernel<T, N, true>, dim3(blocks < most ? blocks : most), block, 0, st, NO_CLUSTER, x, residual, w, q, scales, rows,    \
+                        size, eps);                                                                                                                           \
     }
+        switch (n) {
+            AK_NORM_Q8(1);
+            AK_NORM_Q8(2);
+        }
+        if constexpr (MOST == 8) {
+            switch (n) { AK_NORM_Q8(4); }
+        }
 #undef AK_NORM_Q8
+    } else {
+        // Many rows: a warp each up to 32 values a thread (16384 x 768 f32 13 us, with 64 threads a row 19), but not with a residual, whose
+        // loads want more threads (26 against 32 us); long ones 16 values a thread, or 8 with a residual (16384 x 2048 31 us against
+        // 39 with 8; with a residual 65.2 us against 67.0 with 16).
+        uint32_t n = few ? 1 : residual ? 2 : groups <= 32 * MOST ? cdiv(groups, 32) : 16 / V;
+        if (n == 5 || n == 7) n++;
+        while (groups > n * 1024) n *= 2;
+        const uint32_t tpr = cdiv(groups, n * 32) * 32;
+        const dim3 block(tpr, tpr == 32 && !few ? 4 : 1);
+#define AK_NORM_Q8(N) \
+    case N: return launch_k(norm_q8_kernel<T, N>, dim3(cdiv(rows, block.y)), block, 0, st, NO_CLUSTER, x, residual, w, q, scales, rows, size, eps)
+        switch (n) {
+            AK_NORM_Q8(1);
+            AK_NORM_Q8(2);
+            AK_NORM_Q8(3);
+            AK_NORM_Q8(4);
+        }
+        if constexpr (MOST == 8) {
+            switch (n) {
+                AK_NORM_Q8(6);
+                AK_NORM_Q8(8);
+            }
+        }
+#undef AK_NORM_Q8
+    }
+    set_error("ak_rmsnorm_q8: no kernel for rows of %u", size);
+    return AK_ERR_UNSUPPORTED;
 }
 
 // ============================================================================ split + RoPE + quantised append
-// qkv row of a token: `heads` query heads, kv_heads key heads, kv_heads value heads. A group of HD / 4 lanes (HD = 96: 24 of 32) takes one
-// head: one float4 per lane, its two pairs rotated, the largest magnitude of the head by shuffles inside the group, 4 bytes out.
+// qkv row of a token: `heads` query heads, kv_heads key heads, kv_heads value heads. HD / 4 lanes (HD = 96: 24 of 32) take a head: one
+// float4 each, its two pairs rotated, the largest magnitude of the head by shuffles, 4 bytes out. A block takes one token (several, where
+// their heads do not fill it): position, slot and the lane's RoPE factors are read once for all its heads, 4 of which are in flight at a time.
+constexpr uint32_t AP_THREADS = 256, AP_AHEAD = 4;
+template <int HD> struct ApCfg {
+    static constexpr uint32_t LANES = HD / 4, GROUP = HD == 96 ? 32 : LANES;   // lanes at work / set aside for a head
+    static constexpr uint32_t GROUPS = AP_THREADS / GROUP;
+};
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(AP_THREADS)
 rope_kv_append_q8_kernel(const float* __restrict__ qkv, const float4* __restrict__ rope, uint32_t rope_len, const int32_t* __restrict__ positions,
                          const int32_t* __restrict__ slots, T* __restrict__ q_out, int8_t* __restrict__ k_pool, int8_t* __restrict__ v_pool,
-                         float* __restrict__ k_scales, float* __restrict__ v_scales, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t pool_slots) {
-    constexpr uint32_t LANES = HD / 4, GROUP = HD == 96 ? 32 : LANES;   // lanes at work / lanes set aside for a head
+                         float* __restrict__ k_scales, float* __restrict__ v_scales, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t pool_slots,
+                         uint32_t per_block) {
+    using C = ApCfg<HD>;
     pdl_wait();
     pdl_trigger();
-    const uint32_t total_heads = heads + 2 * kv_heads;
-    const uint64_t item = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) / GROUP;
-    const uint32_t l = threadIdx.x % GROUP;
-    const uint32_t t = (uint32_t)(item / total_heads), h = (uint32_t)(item % total_heads);
-    const bool on = t < tokens && l < LANES;
+    const uint32_t total = heads + 2 * kv_heads, group = threadIdx.x / C::GROUP, l = threadIdx.x % C::GROUP;
+    const uint32_t mine = per_block > 1 ? group / total : 0;   // which of the block's tokens
+    const uint32_t t = blockIdx.x * per_block + mine;
+    uint32_t h = per_block > 1 ? group - mine * total : group;
+    const bool on = t < tokens && mine < per_block && l < C::LANES;
     int32_t pos = -1, slot = -1;
     if (on) { pos = positions[t]; slot = slots[t]; }
     const bool live = on && (uint32_t)pos < rope_len;   // a token at another position is left out
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) {
-        x = *reinterpret_cast<const float4*>(qkv + ((uint64_t)t * total_heads + h) * HD + 4 * l);
-        if (h < heads + kv_heads) {
-            const float4 f = rope[(uint64_t)pos * (HD / 4) + l];   // (cos, sin) of pairs 2l and 2l + 1
-            rope_rotate(x.x, x.y, f.x, f.y, x.x, x.y);
-            rope_rotate(x.z, x.w, f.z, f.w, x.z, x.w);
-        }
-    }
-    uint32_t top = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
+    const float* row = qkv + ((uint64_t)(live ? t : 0) * total) * HD + 4 * (l < C::LANES ? l : 0);
+    float4 f = make_float4(1.f, 0.f, 1.f, 0.f);
+    if (live) f = rope[(uint64_t)pos * (HD / 4) + l];   // (cos, sin) of pairs 2l and 2l + 1
+    const uint64_t block = (uint32_t)slot / Q8_BS, place = (uint32_t)slot % Q8_BS;
+    const bool cached = (uint32_t)slot < pool_slots;
+    // whole blocks go round together: the shuffles want every lane of a group
+    for (uint32_t base = 0; base < total; base += AP_AHEAD * C::GROUPS) {
+        float4 x[AP_AHEAD];
 #pragma unroll
-    for (uint32_t o = GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!live) return;
-    if (h < heads) {
-        T* dst = q_out + ((uint64_t)t * heads + h) * HD + 4 * l;
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(dst) = x;
-        } else {
-            const bf162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
-            *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        for (uint32_t j = 0; j < AP_AHEAD; j++) {
+            x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (live && h + j * C::GROUPS < total) x[j] = *reinterpret_cast<const float4*>(row + (uint64_t)(h + j * C::GROUPS) * HD);
         }
-        return;
+#pragma unroll
+        for (uint32_t j = 0; j < AP_AHEAD; j++) {
+            const uint32_t hj = h + j * C::GROUPS;
+            if (hj < heads + kv_heads) {
+                rope_rotate(x[j].x, x[j].y, f.x, f.y, x[j].x, x[j].y);
+                rope_rotate(x[j].z, x[j].w, f.z, f.w, x[j].z, x[j].w);
+            }
+            if (hj < heads && live) {
+                T* dst = q_out + ((uint64_t)t * heads + hj) * HD + 4 * l;
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<float4*>(dst) = x[j];
+                } else {
+                    const bf162 a = __floats2bfloat162_rn(x[j].x, x[j].y), b = __floats2bfloat162_rn(x[j].z, x[j].w);
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+                }
+            }
+            const bool kv = hj >= heads && hj < total;
+            if (!__any_sync(0xffffffffu, kv)) continue;   // a warp of query heads
+            uint32_t top = max(max(abs_bits(x[j].x), abs_bits(x[j].y)), max(abs_bits(x[j].z), abs_bits(x[j].w)));
+            if constexpr (C::GROUP == 32) {
+                top = __reduce_max_sync(0xffffffffu, top);
+            } else {
+#pragma unroll
+                for (uint32_t o = C::GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            }
+            if (kv && live && cached) {
+                const bool is_v = hj >= heads + kv_heads;
+                const uint64_t at = (block * kv_heads + (hj - heads - (is_v ? kv_heads : 0))) * Q8_BS + place;
+                float inv, s;
+                q8_scale(top, inv, s);
+                *reinterpret_cast<uint32_t*>((is_v ? v_pool : k_pool) + at * HD + 4 * l) = q8_pack4(x[j].x, x[j].y, x[j].z, x[j].w, inv, s == s);
+                if (l == 0) (is_v ? v_scales : k_scales)[at] = s;
+            }
+        }
+        h += AP_AHEAD * C::GROUPS;
+        if (per_block > 1) break;
     }
-    if ((uint32_t)slot >= pool_slots) return;   // not cached
-    const bool is_v = h >= heads + kv_heads;
-    const uint32_t kh = h - heads - (is_v ? kv_heads : 0);
-    const uint64_t at = ((uint64_t)((uint32_t)slot / Q8_BS) * kv_heads + kh) * Q8_BS + (uint32_t)slot % Q8_BS;
-    float inv, s;
-    q8_scale(top, inv, s);
-    *reinterpret_cast<uint32_t*>((is_v ? v_pool : k_pool) + at * HD + 4 * l) = q8_pack4(x.x, x.y, x.z, x.w, inv);
-    if (l == 0) (is_v ? v_scales : k_scales)[at] = s;
 }
 
 // ============================================================================ cached rows as numbers
-// A thread takes 16 bytes of output (VEC values) of the key row and of the value row of one (token, head).
-template <typename T>
-__global__ void __launch_bounds__(256)
+// 16 bytes of output (VEC values) of the key row and of the value row of one (token, head) a thread and turn, RD_AHEAD turns in flight.
+constexpr uint32_t RD_THREADS = 256, RD_AHEAD = 4;
+template <typename T, int HD> struct RdCfg {
+    static constexpr uint32_t VEC = 16 / sizeof(T), CHUNKS = HD / VEC;
+    static constexpr uint32_t ROWS = RD_THREADS * RD_AHEAD / CHUNKS;   // (token, head) rows of a block
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(RD_THREADS)
 kv_read_q8_kernel(const int8_t* __restrict__ k_pool, const int8_t* __restrict__ v_pool, const float* __restrict__ k_scales, const float* __restrict__ v_scales,
-                  const int32_t* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out, uint32_t tokens, uint32_t kv_heads, uint32_t hd,
-                  uint32_t pool_slots) {
-    constexpr uint32_t VEC = 16 / sizeof(T);
+                  const int32_t* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out, uint32_t rows, const Q8Div kv_heads, uint32_t pool_slots) {
+    using C = RdCfg<T, HD>;
     pdl_wait();
     pdl_trigger();
-    const uint32_t chunks = hd / VEC;
-    const uint64_t idx = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (idx >= (uint64_t)tokens * kv_heads * chunks) return;
-    const uint32_t c = (uint32_t)(idx % chunks);
-    const uint64_t th = idx / chunks;
-    const uint32_t h = (uint32_t)(th % kv_heads), t = (uint32_t)(th / kv_heads);
-    const uint32_t slot = (uint32_t)slots[t];
-    const bool have = slot < pool_slots;
-    const uint64_t at = have ? ((uint64_t)(slot / Q8_BS) * kv_heads + h) * Q8_BS + slot % Q8_BS : 0;
+    uint32_t row[RD_AHEAD], words[RD_AHEAD][2][C::VEC / 4];
+    float s[RD_AHEAD][2];
 #pragma unroll
-    for (int side = 0; side < 2; side++) {
-        T* out = side ? v_out : k_out;
-        if (!out) continue;
-        alignas(16) T o[VEC];
-        uint32_t words[VEC / 4];
-        float s = 0.0f;
+    for (uint32_t j = 0; j < RD_AHEAD; j++) {
+        const uint32_t item = j * RD_THREADS + threadIdx.x, c = item % C::CHUNKS;
+        row[j] = blockIdx.x * C::ROWS + item / C::CHUNKS;
+        if (item / C::CHUNKS >= C::ROWS || row[j] >= rows) row[j] = 0xffffffffu;
+        uint32_t slot = 0xffffffffu, h = 0;
+        if (row[j] != 0xffffffffu) {
+            const uint32_t t = kv_heads.of(row[j]);
+            h = row[j] - t * kv_heads.d;
+            slot = (uint32_t)slots[t];
+        }
+        const bool have = slot < pool_slots;
+        const uint64_t at = have ? ((uint64_t)(slot / Q8_BS) * kv_heads.d + h) * Q8_BS + slot % Q8_BS : 0;
 #pragma unroll
-        for (uint32_t i = 0; i < VEC / 4; i++) words[i] = 0;
-        if (have) {
-            const int8_t* src = (side ? v_pool : k_pool) + at * hd + c * VEC;
-            s = (side ? v_scales : k_scales)[at];
-            if constexpr (VEC == 8) {
+        for (int side = 0; side < 2; side++) {
+            s[j][side] = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < C::VEC / 4; i++) words[j][side][i] = 0;
+            if (!have || !(side ? v_out : k_out)) continue;
+            const int8_t* src = (side ? v_pool : k_pool) + at * HD + c * C::VEC;
+            s[j][side] = (side ? v_scales : k_scales)[at];
+            if constexpr (C::VEC == 8) {
                 const uint2 u = *reinterpret_cast<const uint2*>(src);
-                words[0] = u.x; words[1] = u.y;
+                words[j][side][0] = u.x; words[j][side][1] = u.y;
             } else {
-                words[0] = *reinterpret_cast<const uint32_t*>(src);
+                words[j][side][0] = *reinterpret_cast<const uint32_t*>(src);
             }
         }
+    }
 #pragma unroll
-        for (uint32_t i = 0; i < VEC; i++) o[i] = Cvt<T>::from_f((float)(int8_t)(words[i / 4] >> (8 * (i % 4))) * s);
-        *reinterpret_cast<uint4*>(out + idx * VEC) = *reinterpret_cast<const uint4*>(o);
+    for (uint32_t j = 0; j < RD_AHEAD; j++) {
+        const uint32_t c = (j * RD_THREADS + threadIdx.x) % C::CHUNKS;
+        if (row[j] == 0xffffffffu) continue;
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+            T* out = side ? v_out : k_out;
+            if (!out) continue;
+            alignas(16) T o[C::VEC];
+#pragma unroll
+            for (uint32_t i = 0; i < C::VEC; i++) o[i] = Cvt<T>::from_f((float)(int8_t)(words[j][side][i / 4] >> (8 * (i % 4))) * s[j][side]);
+            *reinterpret_cast<uint4*>(out + (uint64_t)row[j] * HD + c * C::VEC) = *reinterpret_cast<const uint4*>(o);
+        }
     }
 }
 
 template <typename T, int HD>
 static int append_q8(cudaStream_t st, const float* qkv, const float* rope, uint32_t rope_len, const int32_t* positions, const int32_t* slots, void* q_out,
                      int8_t* k_pool, int8_t* v_pool, float* k_scales, float* v_scales, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t pool_slots) {
-    constexpr uint32_t GROUP = HD == 96 ? 32 : HD / 4;
-    const uint64_t threads = (uint64_t)tokens * (heads + 2 * kv_heads) * GROUP;
-    AK_REQUIRE(cdiv64(threads, 256) <= 0x7fffffffu, AK_ERR_UNSUPPORTED, "ak_rope_kv_append_q8: %u tokens x %u heads are too many for one call", tokens,
-               heads + 2 * kv_heads);
-    return launch_k(rope_kv_append_q8_kernel<T, HD>, dim3((unsigned)cdiv64(threads, 256)), dim3(256), 0, st, NO_CLUSTER, qkv,
+    const uint32_t total = heads + 2 * kv_heads, per_block = total >= ApCfg<HD>::GROUPS ? 1 : ApCfg<HD>::GROUPS / total;
+    return launch_k(rope_kv_append_q8_kernel<T, HD>, dim3(cdiv(tokens, per_block)), dim3(AP_THREADS), 0, st, NO_CLUSTER, qkv,
                     reinterpret_cast<const float4*>(rope), rope_len, positions, slots, (T*)q_out, k_pool, v_pool, k_scales, v_scales, tokens, heads, kv_heads,
-                    pool_slots);
+                    pool_slots, per_block);
+}
+
+template <typename T, int HD>
+static int read_q8(cudaStream_t st, const int8_t* k_pool, const int8_t* v_pool, const float* k_scales, const float* v_scales, const int32_t* slots, void* k_out,
+                   void* v_out, uint32_t tokens, uint32_t kv_heads, uint32_t pool_slots) {
+    const uint32_t rows = tokens * kv_heads;
+    return launch_k(kv_read_q8_kernel<T, HD>, dim3(cdiv(rows, RdCfg<T, HD>::ROWS)), dim3(RD_THREADS), 0, st, NO_CLUSTER, k_pool, v_pool, k_scales, v_scales,
+                    slots, (T*)k_out, (T*)v_out, rows, Q8Div(kv_heads), pool_slots);
 }
 
 // The cache's own numbers, checked alike by everything that touches it.
@@ -361,6 +563,7 @@ int ak_rope_kv_append_q8(void* stream, const float* qkv, const float* rope_table
     AK_REQUIRE(rope_len >= 1, AK_ERR_INVALID_ARG, "%s: the RoPE table is empty", who);
     AK_REQUIRE(q8_aligned(qkv, 16) && q8_aligned(rope_table, 16) && q8_aligned(q_out, 16) && q8_aligned(positions, 4) && q8_aligned(slots, 4),
                AK_ERR_INVALID_ARG, "%s: qkv, q_out and the RoPE table must be 16-byte aligned, positions and slots 4-byte", who);
+    AK_REQUIRE(tokens <= 0x7fffffffu, AK_ERR_UNSUPPORTED, "%s: %u tokens are too many for one call", who, tokens);
     if (tokens == 0) return AK_OK;
     AK_TRY(q8_check_here(k_pool, who));
 #define AK_APPEND_Q8(T, HD)                                                                                                                              \
@@ -387,13 +590,18 @@ int ak_kv_read_q8(void* stream, const int8_t* k_pool, const int8_t* v_pool, cons
     AK_REQUIRE(q8_aligned(k_out, 16) && q8_aligned(v_out, 16) && q8_aligned(slots, 4), AK_ERR_INVALID_ARG, "%s: the outputs must be 16-byte aligned, slots 4-byte", who);
     if (tokens == 0) return AK_OK;
     AK_TRY(q8_check_here(k_pool, who));
-    const uint64_t threads = (uint64_t)tokens * kv_heads * (head_dim / (out_dtype == AK_F32 ? 4 : 8));
-    AK_REQUIRE(cdiv64(threads, 256) <= 0x7fffffffu, AK_ERR_UNSUPPORTED, "%s: %u tokens x %u heads are too many for one call", who, tokens, kv_heads);
-    const dim3 grid((unsigned)cdiv64(threads, 256));
-    if (out_dtype == AK_F32)
-        return launch_k(kv_read_q8_kernel<float>, grid, dim3(256), 0, as_stream(stream), NO_CLUSTER, k_pool, v_pool, k_scales, v_scales, slots, (float*)k_out,
-                        (float*)v_out, tokens, kv_heads, head_dim, pool_blocks * Q8_BS);
-    return launch_k(kv_read_q8_kernel<bf16>, grid, dim3(256), 0, as_stream(stream), NO_CLUSTER, k_pool, v_pool, k_scales, v_scales, slots, (bf16*)k_out,
-                    (bf16*)v_out, tokens, kv_heads, head_dim, pool_blocks * Q8_BS);
+    AK_REQUIRE((uint64_t)tokens * kv_heads <= 0x7fffffffu, AK_ERR_UNSUPPORTED, "%s: %u tokens x %u heads are too many for one call", who, tokens, kv_heads);
+#define AK_READ_Q8(T, HD) return read_q8<T, HD>(as_stream(stream), k_pool, v_pool, k_scales, v_scales, slots, k_out, v_out, tokens, kv_heads, pool_blocks * Q8_BS)
+#define AK_READ_Q8_HD(T)                         \
+    switch (head_dim) {                          \
+        case 32: AK_READ_Q8(T, 32);              \
+        case 64: AK_READ_Q8(T, 64);              \
+        case 96: AK_READ_Q8(T, 96);              \
+        default: AK_READ_Q8(T, 128);             \
+    }
+    if (out_dtype == AK_F32) { AK_READ_Q8_HD(float) }
+    AK_READ_Q8_HD(bf16)
+#undef AK_READ_Q8_HD
+#undef AK_READ_Q8
 }
 }

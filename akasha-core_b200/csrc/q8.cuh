@@ -14,6 +14,19 @@ int q8_check_here(const void* p, const char* who);
 int q8_check_cache(const char* who, const void* k_pool, const void* v_pool, const void* k_scales, const void* v_scales, uint32_t heads, uint32_t kv_heads,
                    uint32_t head_dim, uint32_t block_size, uint32_t dtype, uint32_t pool_blocks);
 
+// n / d for n below 2^31: (n * mul) >> (31 + shift) with mul = floor(2^(31 + shift) / d) + 1 and 2^shift >= d, whose excess over 2^(31 + shift) / d is
+// at most 1, an error of n / 2^(31 + shift) < 2^-shift <= 1 / d.
+struct Q8Div {
+    uint32_t d, mul, shift;
+    Q8Div(uint32_t div) : d(div), shift(0) {
+        while ((1ull << shift) < d) shift++;
+        mul = (uint32_t)((1ull << (31 + shift)) / d + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> (31 + shift)); }
+#endif
+};
+
 static inline bool q8_aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Head sizes that the cache's kernels are built for.
@@ -28,15 +41,23 @@ static inline bool q8_head_dim_ok(uint32_t hd) { return hd == 32 || hd == 64 || 
 constexpr float Q8_ZERO = 1e-30f;
 __device__ __forceinline__ void q8_scale(uint32_t top_bits, float& inv, float& s) {
     const float top = __uint_as_float(top_bits);
+    float r;   // 128 / top: the factor keeps the reciprocal of the largest values away from what the approximation flushes to 0
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top * 0.0078125f));
+    inv = r * 0.9921875f;        // 127 / top to 3 * 2^-24, where a division took fifteen instructions
+    s = top * (1.0f / 127.0f);   // the constant is off by 2^-28 of its value
+    if (top < Q8_ZERO) { inv = 0.0f; s = 0.0f; }
     if (top_bits >= 0x7f800000u) { inv = 0.0f; s = __uint_as_float(0x7fc00000u); }
-    else if (top < Q8_ZERO) { inv = 0.0f; s = 0.0f; }
-    else { inv = 127.0f / top; s = top / 127.0f; }
 }
-// |y inv| <= 127 (1 + 2^-23): the nearest integer never leaves -127..127. (inv = 0: infinity times 0 is NaN, which converts to 0.)
-__device__ __forceinline__ uint32_t q8_of(float y, float inv) { return (uint32_t)__float2int_rn(y * inv) & 0xffu; }
-__device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d, float inv) {
-    return q8_of(a, inv) | (q8_of(b, inv) << 8) | (q8_of(c, inv) << 16) | (q8_of(d, inv) << 24);
+// The four integers nearest to y inv, |y inv| <= 127 (1 + 2^-23), as bytes. Adding 1.5 * 2^23 leaves the nearest integer in a float's low bits; one
+// that is not finite (times inv = 0) would leave any bits there: `ok` = the row's scale is a number.
+__device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d, float inv, bool ok) {
+    constexpr float M = 12582912.0f;
+    const uint32_t ia = __float_as_uint(fmaf(a, inv, M)), ib = __float_as_uint(fmaf(b, inv, M));
+    const uint32_t ic = __float_as_uint(fmaf(c, inv, M)), id = __float_as_uint(fmaf(d, inv, M));
+    const uint32_t v = __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+    return ok ? v : 0u;
 }
+__device__ __forceinline__ int8_t q8_of(float y, float inv, bool ok) { return ok ? (int8_t)__float2int_rn(y * inv) : (int8_t)0; }
 __device__ __forceinline__ bool q8_aligned_dev(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 

@@ -313,11 +313,12 @@ AK_API int ak_kv_read_q8(void* stream, const int8_t* k_pool, const int8_t* v_poo
 /* Attention of the newest q_len tokens of every sequence over the cache (decode: q_len = 1; drafted tokens or a chunk of a prompt: more):
  *   q, out [rows * q_len, heads * head_dim] (dtype); query i of a row is at position kv_lens[row] - q_len + i and sees the positions up to its
  *   own (kv_lens counts the new tokens, which are in the cache already). Lengths are cut at 16 * max_blocks_per_seq; a query with no
- *   position to see gives zeros. block_tables int32 [rows, max_blocks_per_seq], entries past a sequence's end are not read; the positions of a block id
- *   outside the pool are left out. scale multiplies q . k.
+ *   position to see gives zeros. block_tables int32 [rows, max_blocks_per_seq], entries past a sequence's end are not used; the positions of a
+ *   block id outside the pool are left out. scale multiplies q . k.
  *   n_splits: CTAs that share a sequence, as one thread-block cluster; 0 = the library's choice, else 1 to 16 (rounded down to a power of two).
- * f32 arithmetic throughout (queries and softmax weights as two f16 parts), but for bf16 with more than 8 query rows per kv head
- * (q_len * heads / kv_heads), where weights are rounded to f16. A weight below 2^-38 of its sequence's largest weight-times-scale may count as 0. */
+ * Sums, maxima and softmax weights are f32. A query is held as integers of 24 bits (f32) or 16 bits (bf16) of its head's largest value (one under
+ * 1e-30 counts as 0); the weights of V have 22 bits, or, for bf16 with more than 4 query rows per kv head (q_len * heads / kv_heads), 11. A weight below
+ * 2^-29 of its sequence's largest weight-times-scale may count as 0. */
 typedef struct ak_attn_q8_params {
     uint32_t rows, q_len, heads, kv_heads, head_dim, block_size, max_blocks_per_seq;
     float scale;
