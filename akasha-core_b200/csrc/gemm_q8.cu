@@ -5,7 +5,8 @@
 // element), accumulators in TMEM, read back with tcgen05.ld. A sum of k products is at most 2^14 k in size: exact for k up to 131056 (the
 // largest multiple of 16 below 2^17). It is converted to f32 (one rounding above 2^24), multiplied by the row's and then the column's scale.
 //
-// Two kernels: a CTA pair on 256 x 256 tiles, persistent, for large m; one CTA per tile, K split over the CTAs of a cluster, for the rest.
+// Two kernels: a CTA pair on 256 x 256 tiles, persistent, for large m; one CTA per tile of 128 rows and 16 to 256 columns, K split over the CTAs of a
+// cluster, for the rest.
 // Integer sums do not depend on their order: a row's result is the same whatever shares the launch, split or not.
 //
 // Nothing is read before griddepcontrol.wait: the weights may be the result of the kernel just before (ak_rmsnorm_q8 quantises them as well).
@@ -51,13 +52,13 @@ __device__ __forceinline__ void col_scales(const float* w, uint32_t col, uint32_
 // grid = (n tiles, m tiles, ks), cluster = (1, 1, ks): the CTAs of a cluster take a part of K each, push the column slice that a peer owns
 // into its shared memory, and every one adds up and stores its own slice.
 // Warp 0 = TMA producer, warp 1 = MMA issuer (+ TMEM), warps 2-5 = epilogue, one TMEM lane quadrant each.
-template <int BN, int EPI, bool SPLIT>
+template <int EPI, bool SPLIT>
 __global__ void __launch_bounds__(I8_THREADS)
 gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmEpi ep, const I8Scales sc, uint32_t m, uint32_t n,
-               uint32_t k, uint32_t stages, uint32_t tmem_cols, uint32_t a_rows, uint32_t a_box) {
-    // a_rows: rows of an activation slot. The MMA reads 128 rows from its start; what follows the box feeds accumulator rows that are never
-    // stored.
-    constexpr uint32_t B_BYTES = BN * I8_KB;
+               uint32_t k, uint32_t bn, uint32_t stages, uint32_t tmem_cols, uint32_t a_rows, uint32_t a_box) {
+    // bn: columns of the tile, a multiple of 16 up to 256. a_rows: rows of an activation slot. The MMA reads 128 rows from its start; what
+    // follows the box feeds accumulator rows that are never stored.
+    const uint32_t B_BYTES = bn * I8_KB;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[I8_MAX_STAGES], empty_bar[I8_MAX_STAGES], acc_bar, xch_bar;
     __shared__ uint32_t tmem_base_sm, fail_flag;
@@ -68,9 +69,9 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     const uint32_t a_bytes = a_rows * I8_KB, stage_tx = a_box * I8_KB + B_BYTES;
     uint8_t* const b_base = smem + (size_t)stages * a_bytes;
     const uint32_t overrun = (I8_M - a_rows) * I8_KB, b_total = stages * B_BYTES;
-    int32_t* red = reinterpret_cast<int32_t*>(b_base + b_total + (overrun > b_total ? overrun - b_total : 0u));   // exchange buffer [ks][a_rows][BN / ks]
+    int32_t* red = reinterpret_cast<int32_t*>(b_base + b_total + (overrun > b_total ? overrun - b_total : 0u));   // exchange buffer [ks][a_rows][bn / ks]
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const uint32_t m0 = blockIdx.y * I8_M, n0 = blockIdx.x * BN;
+    const uint32_t m0 = blockIdx.y * I8_M, n0 = blockIdx.x * bn;
     const uint32_t kb_total = (k + I8_KB - 1) / I8_KB, per = (kb_total + ks - 1) / ks;
     const uint32_t kb_begin = min(rank * per, kb_total), num_kb = min(per, kb_total - kb_begin);
 
@@ -80,8 +81,8 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         mbar_init(&xch_bar, 1);
         fail_flag = 0;
         mbar_fence_init();
-        // the slices that the peers will push: BN / ks columns of every valid row from each of them (armed before the start barrier)
-        if (SPLIT) mbar_expect_tx(&xch_bar, (ks - 1) * min(m - m0, I8_M) * ((uint32_t)BN / ks) * 4u);
+        // the slices that the peers will push: bn / ks columns of every valid row from each of them (armed before the start barrier)
+        if (SPLIT) mbar_expect_tx(&xch_bar, (ks - 1) * min(m - m0, I8_M) * (bn / ks) * 4u);
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
     }
@@ -110,14 +111,14 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             }
         }
     } else if (warp == 1) {
-        constexpr uint32_t idesc = make_idesc_i8(I8_M, BN);
+        const uint32_t idesc = make_idesc_i8(I8_M, bn);
         uint32_t s = 0, ph = 0;
         const uint64_t da0 = make_smem_desc(smem_u32(smem)), db0 = make_smem_desc(smem_u32(b_base));
         const uint32_t da_step = a_bytes >> 4;
         for (uint32_t i = 0; i < num_kb; i++) {
             if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph))) { if (lane == 0) atomicExch(&fail_flag, 2u); break; }
             tc_fence_after();
-            const uint64_t da = da0 + s * da_step, db = db0 + s * (uint32_t)(B_BYTES >> 4);
+            const uint64_t da = da0 + s * da_step, db = db0 + s * (B_BYTES >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (uint32_t kk = 0; kk < I8_KB / 32; kk++)   // 32 values = 32 bytes along K: +2 in the descriptor's address field
@@ -134,33 +135,35 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     const uint32_t quad = warp & 3u, trow = quad * 32 + lane, row = m0 + trow;
     const bool vec = q8_aligned_dev(sc.w);
     bool got = true;
+    float sw[16];   // the next columns' scales are on their way while these are used
+    const float sa = (warp >= 2 && row < m) ? sc.a[row] : 0.0f;
     if (warp >= 2) {
+        if (!SPLIT) col_scales<16>(sc.w, n0, n, vec, sw);
         got = mbar_wait(&acc_bar, 0);
         if (!got && lane == 0) atomicExch(&fail_flag, 3u);
         got = __all_sync(0xffffffffu, got);
         tc_fence_after();
     }
-    const float sa = (warp >= 2 && row < m) ? sc.a[row] : 0.0f;
     if (!SPLIT) {
         if (warp >= 2 && got) {
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < (uint32_t)BN; c0 += 16) {
+            for (uint32_t c0 = 0; c0 < bn; c0 += 16) {
                 uint32_t r[16];
-                float v[16], sw[16];
+                float v[16];
                 tmem_ld16(tmem_base + ((quad * 32u) << 16) + c0, r);
-                col_scales<16>(sc.w, n0 + c0, n, vec, sw);
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 16; j++) v[j] = (float)(int32_t)r[j] * sa * sw[j];
+                if (c0 + 16 < bn) col_scales<16>(sc.w, n0 + c0 + 16, n, vec, sw);
                 epi_store16<EPI>(ep, row, row < m, n0 + c0, v, n, lane);
             }
         }
     } else {
-        const uint32_t SL = (uint32_t)BN / ks;   // columns of a slice, a multiple of 4
+        const uint32_t SL = bn / ks;   // columns of a slice, a multiple of 4
         cluster_wait_all();                      // every peer runs
         if (warp >= 2 && got) {
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < (uint32_t)BN; c0 += 16) {
+            for (uint32_t c0 = 0; c0 < bn; c0 += 16) {
                 uint32_t r[16];
                 if (num_kb > 0) {
                     tmem_ld16(tmem_base + ((quad * 32u) << 16) + c0, r);
@@ -192,9 +195,9 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                         acc.x += p.x; acc.y += p.y; acc.z += p.z; acc.w += p.w;
                     }
                     const uint32_t col = n0 + rank * SL + j;
-                    float sw[4];
-                    col_scales<4>(sc.w, col, n, vec, sw);
-                    const float v[4] = {(float)acc.x * sa * sw[0], (float)acc.y * sa * sw[1], (float)acc.z * sa * sw[2], (float)acc.w * sa * sw[3]};
+                    float s4[4];
+                    col_scales<4>(sc.w, col, n, vec, s4);
+                    const float v[4] = {(float)acc.x * sa * s4[0], (float)acc.y * sa * s4[1], (float)acc.z * sa * s4[2], (float)acc.w * sa * s4[3]};
                     epi_store<EPI, 4>(ep, row, col, v, n);
                 }
             }
@@ -210,6 +213,11 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 }
 
 // ============================================================================ CTA pair
+// Measured (graph of launches): 16384 x 8192 x 2048 184 us = 2990 TOPS with bf16 results, 192 with SiLU, 4001 x 2048 x 8192 added to f32 50 us (128 tiles
+// are two turns of 74 pairs, the second one not full); the tensor pipe is busy for 75 % of the cycles, and the power limit takes
+// a fifth of the clock in longer runs. What feeds it is the L2: a K block of 64 KB takes a pair 0.39 us, its MMAs 0.27. Below K = 1024 the results
+// bound it, 3 us a tile (16 epilogue warps and five stages instead of 8 and six: the same there, 4 % slower for long K).
+//
 // A cluster of two CTAs walks over [256 x 256] tiles: each stages its 128 rows of A and its half (128 rows) of the weight tile per K block, the
 // leader issues MMAs of 256 x 256 x 32 that read both CTAs' shared memory, rows 0-127 accumulate in its TMEM and rows 128-255 in the peer's.
 // Two accumulator buffers of 256 columns: the epilogue drains one tile while the MMAs of the next run.
@@ -217,6 +225,7 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 //   acc_full[b]   one per CTA, committed after a tile's last MMA;             acc_empty[b]  leader's, 16 arrivals (8 epilogue warps of each CTA).
 constexpr int I8P_BN = 256;
 constexpr int I8P_EPI_WARPS = 8;
+constexpr int I8P_EPI_COLS = I8P_BN / (I8P_EPI_WARPS / 4);   // of a tile, for each of a lane quadrant's warps
 constexpr int I8P_THREADS = 128 + I8P_EPI_WARPS * 32;   // the first warpgroup holds the TMA and the MMA warp
 constexpr uint32_t I8P_A_BYTES = I8_M * I8_KB, I8P_STAGE = I8P_A_BYTES + (I8P_BN / 2) * I8_KB;
 constexpr uint32_t I8P_OUT_WARP = 32 * 128;             // an epilogue warp's staged piece: 32 rows x 128 bytes
@@ -318,7 +327,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     } else if (warp >= 4) {
         // Two warps per lane quadrant, half of the columns each. `tma_out`: pieces of 32 rows x 128 bytes go through a swizzled buffer and
         // leave as TMA stores (or adds into f32); otherwise (pitch of C not a multiple of 16 bytes) from registers.
-        const uint32_t quad = warp & 3u, half = (warp - 4) >> 2;
+        const uint32_t quad = warp & 3u, part = (warp - 4) >> 2;
         constexpr bool OUT_BF16 = (EPI == AK_EPI_STORE_BF16 || EPI == AK_EPI_SILU_BF16);
         constexpr uint32_t CW = OUT_BF16 ? 64 : 32;
         uint8_t* const stage_sm = smem + (size_t)stages * I8P_STAGE + (size_t)(warp - 4) * I8P_OUT_WARP;
@@ -326,27 +335,29 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         uint32_t tc = 0;
         for (uint32_t t = pair; t < tiles_total; t += n_pairs, tc++) {
             const uint32_t row0 = ((t / tiles_n) * 2 + rank) * I8_M + quad * 32, row = row0 + lane;
-            const uint32_t n0 = (t % tiles_n) * I8P_BN + half * (I8P_BN / 2);
-            const uint32_t acc0 = tmem_base + ((quad * 32u) << 16) + (tc & 1u) * I8P_BN + half * (I8P_BN / 2);
+            const uint32_t n0 = (t % tiles_n) * I8P_BN + part * I8P_EPI_COLS;
+            const uint32_t acc0 = tmem_base + ((quad * 32u) << 16) + (tc & 1u) * I8P_BN + part * I8P_EPI_COLS;
             const float sa = row < m ? sc.a[row] : 0.0f;
+            float sw[32];   // the next columns' scales are on their way while these are used
+            col_scales<32>(sc.w, n0, n, vec, sw);
             bool got = mbar_wait(&acc_full[tc & 1u], (tc >> 1) & 1u);
             if (!got && lane == 0) atomicExch(&fail_flag, 3u);
             if (!__all_sync(0xffffffffu, got)) break;
             tc_fence_after();
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < (uint32_t)I8P_BN / 2; c0 += 32) {
+            for (uint32_t c0 = 0; c0 < (uint32_t)I8P_EPI_COLS; c0 += 32) {
                 uint32_t r[32];
-                float v[32], sw[32];
+                float v[32];
                 tmem_ld32(acc0 + c0, r);
-                col_scales<32>(sc.w, n0 + c0, n, vec, sw);
                 tmem_ld_wait();
-                if (c0 + 32 == (uint32_t)I8P_BN / 2) {   // this warp has read its part: the buffer may be written again
+                if (c0 + 32 == (uint32_t)I8P_EPI_COLS) {   // this warp has read its part: the buffer may be written again
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[tc & 1u]), 0));
                 }
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = (float)(int32_t)r[j] * sa * sw[j];
+                if (c0 + 32 < (uint32_t)I8P_EPI_COLS) col_scales<32>(sc.w, n0 + c0 + 32, n, vec, sw);
                 const uint32_t col = n0 + (OUT_BF16 ? (c0 & ~32u) : c0);   // first column of the staged piece
                 // a store is clipped at n in whole 16-byte units only: a ragged last piece is stored from registers
                 if (!tma_out || (col + CW > n && (n * (OUT_BF16 ? 2u : 4u)) % 16u != 0)) {
@@ -404,9 +415,10 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
 // ============================================================================ launch
 constexpr uint32_t I8_SMEM_TWO = 112 * 1024;    // two CTAs fit one SM below this
+constexpr uint32_t I8_SMEM_ONE = 220 * 1024;
 constexpr uint32_t I8_SMEM_PAIR = 226 * 1024;
 
-struct I8Plan { uint32_t bn, ks, stages; };
+struct I8Plan { uint32_t bn, ks, stages; };   // bn = 0: the pair kernel
 
 // Rows of the activation box: a small batch fills only part of the 128-row tile, rows that the box does not fetch cost nothing.
 static uint32_t i8_box_rows(uint32_t m) { return m >= I8_M ? I8_M : (m > 64 ? m : (m > 32 ? 64 : (m > 16 ? 32 : 16))); }
@@ -416,30 +428,44 @@ static size_t i8_smem(uint32_t stages, uint32_t bn, uint32_t a_rows, bool split)
     return (size_t)stages * (a_rows + bn) * I8_KB + (overrun > b_total ? overrun - b_total : 0) + (split ? (size_t)a_rows * bn * 4 : 0) + 1024;
 }
 
+// Stages of the ring: what is left of an SM, or of half of one, up to the whole part of K.
+static uint32_t i8_stages(uint32_t bn, uint32_t ks, uint32_t per, uint32_t a_rows, uint64_t ctas) {
+    const size_t room = ctas <= B200_SMS ? I8_SMEM_ONE : I8_SMEM_TWO, stage = (a_rows + bn) * I8_KB, fixed = i8_smem(0, bn, a_rows, ks > 1);
+    uint32_t st = fixed < room ? (uint32_t)((room - fixed) / stage) + (uint32_t)((I8_M - a_rows) / bn) : 0;   // weight slots double as the overrun
+    if (st > I8_MAX_STAGES) st = I8_MAX_STAGES;
+    if (st > per) st = per;
+    while (st > 1 && i8_smem(st, bn, a_rows, ks > 1) > room) st--;
+    return st;
+}
+
+// The shortest of the tile widths, K splits and the pair kernel by what a launch takes, in us. Fitted to 250 measurements of 26 shapes from
+// 1 x 2304 x 768 to 2048^3 and 1500 x 1000 x 4000 (a graph of launches, weights of three sets); over these the choice loses 1.2 % on average
+// against the best of all, 10 % at most (64 x 6144 x 2048: 7.9 us with tiles of 32 columns, 7.2 with 48).
+//   tile   2.1, the epilogue 0.01 a column, and per K block of b KB (activation and weight tile) 0.17 + b / 168, the rate of one TMA stream
+//          from L2; two CTAs on an SM share 121 KB/us, and every further pair of them starts anew. A split adds its exchange.
+//   pair   3.8, and 0.40 per K block of the 74 pairs.
+//   Weights come from HBM at 5.5 MB/us at most.
 static I8Plan i8_plan(uint32_t m, uint32_t n, uint32_t k, bool allow_split) {
     const uint32_t kb = cdiv(k, I8_KB), mt = cdiv(m, I8_M), ar = i8_slot_rows(m);
-    I8Plan p{16, 1, 1};
-    if (m > I8_M || cdiv(n, 64) > 2 * B200_SMS) {
-        // tiles as wide as still leave every SM one
-        p.bn = 16;
-        for (uint32_t bn : {256u, 128u, 64u, 32u})
-            if ((uint64_t)mt * cdiv(n, bn) >= B200_SMS) { p.bn = bn; break; }
-    } else {
-        // one wave of up to two CTAs per SM with the shortest chain of K blocks; more, narrower CTAs where that ties
-        uint32_t best_per = ~0u, best_ctas = 0;
-        for (uint32_t bn : {16u, 32u, 64u})
-            for (uint32_t ks : {1u, 2u, 4u, 8u}) {
-                if (ks > 1 && (!allow_split || ks * 2 > kb || (bn / ks) % 4 != 0)) continue;
-                if (ks > 1 && kb <= 8 && cdiv(n, 16) * 2 > B200_SMS) continue;   // a short chain is split only where SMs would stay idle
-                const uint32_t per = cdiv(kb, ks), ctas = cdiv(n, bn) * ks;
-                if (ks > 1 && (ks - 1) * per >= kb) continue;
-                if (ctas > 2 * B200_SMS && !(bn == 64 && ks == 1)) continue;
-                if (per < best_per || (per == best_per && ctas > best_ctas)) { best_per = per; best_ctas = ctas; p.bn = bn; p.ks = ks; }
-            }
+    const float rows = (float)(m < I8_M ? m : I8_M), stream = (float)n * k / 5.5e6f;
+    I8Plan p{};
+    float best = 1e30f;
+    if (m > I8_M && n > 128) best = 3.8f + (float)cdiv64((uint64_t)cdiv(m, 2 * I8_M) * cdiv(n, I8P_BN), B200_SMS / 2) * kb * 0.40f;
+    for (uint32_t ks = 1; ks <= (allow_split ? 8u : 1u); ks *= 2) {
+        const uint32_t per = cdiv(kb, ks), unit = ks > 4 ? 32 : 16;   // a slice of bn / ks columns is whole groups of 4
+        if (ks > 1 && (ks - 1) * per >= kb) break;                    // every CTA of a cluster gets work
+        for (uint32_t bn = unit; bn <= 256 && bn < n + 16; bn += bn < 128 ? unit : 32) {
+            const uint64_t ctas = (uint64_t)mt * cdiv(n, bn) * ks, turns = (ctas + 2 * B200_SMS - 1) / (2 * B200_SMS);
+            if (ks > 1 && i8_stages(bn, ks, per, ar, ctas) < (per < 4 ? per : 4)) continue;   // the exchange buffer leaves no ring
+            const float b = (float)(ar + bn) * I8_KB * 1e-3f, one = 0.17f + b / 168.0f, two = b / 60.5f;
+            const float load = per * (ctas <= B200_SMS ? one : (float)turns * (one > two ? one : two));
+            float t = 2.1f + 0.01f * bn + (float)(turns - 1) * 0.9f + (load > stream ? load + 0.15f * stream : stream + 0.15f * load);
+            if (ks > 1) t += 0.8f + rows * bn * 4e-3f * (float)(ks - 1) / (float)ks / 7.9f;
+            if (t < best) { best = t; p.bn = bn; p.ks = ks; }
+        }
     }
-    const uint32_t per = cdiv(kb, p.ks);
-    p.stages = per < I8_MAX_STAGES ? per : I8_MAX_STAGES;
-    while (p.stages > 1 && i8_smem(p.stages, p.bn, ar, p.ks > 1) > I8_SMEM_TWO) p.stages--;
+    if (!p.bn) return p;
+    p.stages = i8_stages(p.bn, p.ks, cdiv(kb, p.ks), ar, (uint64_t)mt * cdiv(n, p.bn) * p.ks);
     return p;
 }
 
@@ -455,22 +481,23 @@ static int i8_allow_smem(K* kernel, bool* set, uint32_t bytes) {
     return AK_OK;
 }
 
-template <int BN, int EPI, bool SPLIT>
+template <int EPI, bool SPLIT>
 static int i8_launch_tile(cudaStream_t st, const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmEpi& ep, const I8Scales& sc, uint32_t m, uint32_t n, uint32_t k,
                           const I8Plan& p) {
     static bool set[64] = {};
-    AK_TRY(i8_allow_smem(gemm_q8_kernel<BN, EPI, SPLIT>, set, I8_SMEM_TWO));
+    AK_TRY(i8_allow_smem(gemm_q8_kernel<EPI, SPLIT>, set, I8_SMEM_ONE));
     const uint32_t ar = i8_slot_rows(m);
     uint32_t cols = 32;
-    while (cols < (uint32_t)BN) cols *= 2;
-    return launch_k(gemm_q8_kernel<BN, EPI, SPLIT>, dim3(cdiv(n, BN), cdiv(m, I8_M), p.ks), dim3(I8_THREADS), i8_smem(p.stages, BN, ar, SPLIT), st,
-                    dim3(1, 1, p.ks), tmA, tmB, ep, sc, m, n, k, p.stages, cols, ar, i8_box_rows(m));
+    while (cols < p.bn) cols *= 2;
+    return launch_k(gemm_q8_kernel<EPI, SPLIT>, dim3(cdiv(n, p.bn), cdiv(m, I8_M), p.ks), dim3(I8_THREADS), i8_smem(p.stages, p.bn, ar, SPLIT), st,
+                    dim3(1, 1, p.ks), tmA, tmB, ep, sc, m, n, k, p.bn, p.stages, cols, ar, i8_box_rows(m));
 }
 
 template <int EPI>
 static int i8_launch_epi(cudaStream_t st, const void* a, const void* wt, const GemmEpi& ep, const I8Scales& sc, uint32_t m, uint32_t n, uint32_t k) {
     CUtensorMap tmA, tmB;
-    if (m >= 1024 && n >= 256) {
+    const I8Plan p = i8_plan(m, n, k, ep.ldc % 4 == 0);
+    if (!p.bn) {
         static bool set[64] = {};
         AK_TRY(i8_allow_smem(gemm_q8_pair_kernel<EPI>, set, I8_SMEM_PAIR));
         constexpr uint32_t OUT = I8P_EPI_WARPS * I8P_OUT_WARP, STAGES = (I8_SMEM_PAIR - 1024 - OUT) / I8P_STAGE;
@@ -485,25 +512,9 @@ static int i8_launch_epi(cudaStream_t st, const void* a, const void* wt, const G
         return launch_k(gemm_q8_pair_kernel<EPI>, dim3(2 * pairs), dim3(I8P_THREADS), STAGES * I8P_STAGE + OUT + 1024, st, dim3(2, 1, 1), tmA, tmB, tmC, ep, sc, m,
                         n, k, STAGES, tiles_n, tiles, tma_out);
     }
-    const I8Plan p = i8_plan(m, n, k, ep.ldc % 4 == 0);
     AK_TRY(make_tmap_2d(&tmA, a, 2, k / 2, m, k, I8_KB / 2, i8_box_rows(m), TMA_SWIZZLE_128B));
     AK_TRY(make_tmap_2d(&tmB, wt, 2, k / 2, n, k, I8_KB / 2, p.bn, TMA_SWIZZLE_128B));
-#define AK_TILE(BN, SPLIT) return i8_launch_tile<BN, EPI, SPLIT>(st, tmA, tmB, ep, sc, m, n, k, p)
-    if (p.ks > 1) {
-        switch (p.bn) {
-            case 64: AK_TILE(64, true);
-            case 32: AK_TILE(32, true);
-            default: AK_TILE(16, true);
-        }
-    }
-    switch (p.bn) {
-        case 256: AK_TILE(256, false);
-        case 128: AK_TILE(128, false);
-        case 64: AK_TILE(64, false);
-        case 32: AK_TILE(32, false);
-        default: AK_TILE(16, false);
-    }
-#undef AK_TILE
+    return p.ks > 1 ? i8_launch_tile<EPI, true>(st, tmA, tmB, ep, sc, m, n, k, p) : i8_launch_tile<EPI, false>(st, tmA, tmB, ep, sc, m, n, k, p);
 }
 
 int gemm_q8_status(unsigned int* out) {
