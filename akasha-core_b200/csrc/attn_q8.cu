@@ -398,9 +398,9 @@ attn_decode_q8_kernel(const AqArgs a) {
             }
             // A score more than 8 above its row's reference, or a value scale that the weights' power of two does not cover yet. (In a tile that not
             // every row sees to its end, also by what nobody sees: the branch looks again.)
-            if (__any_sync(0xffffffffu, most > 8.0f || fmaxf(va, vb) >= pow2i(v_exp))) {
+            if (__any_sync(0xffffffffu, most > 8.0f || fmaxf(fabsf(va), fabsf(vb)) >= pow2i(v_exp))) {
                 const int32_t pa = pos0 + (int32_t)g, pb = pa + 8;
-                float vtop = fmaxf(va < INFINITY && pa < lim_max ? va : 0.0f, vb < INFINITY && pb < lim_max ? vb : 0.0f);
+                float vtop = fmaxf(fabsf(va) < INFINITY && pa < lim_max ? fabsf(va) : 0.0f, fabsf(vb) < INFINITY && pb < lim_max ? fabsf(vb) : 0.0f);
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
                 const int ve = (int)(__float_as_uint(vtop) >> 23) - 126;   // vtop < 2^ve
@@ -645,7 +645,8 @@ extern "C" int ak_attn_decode_paged_q8(void* stream, const void* q, const int8_t
     AK_TRY(q8_check_cache(who, k_pool, v_pool, k_scales, v_scales, p.heads, p.kv_heads, p.head_dim, p.block_size, p.dtype, p.pool_blocks));
     AK_REQUIRE(q8_aligned(q, 16) && q8_aligned(out, 16) && q8_aligned(block_tables, 4) && q8_aligned(kv_lens, 4), AK_ERR_INVALID_ARG,
                "%s: q and out must be 16-byte aligned, tables and lengths 4-byte", who);
-    AK_REQUIRE(p.q_len >= 1 && p.q_len <= 65536, AK_ERR_INVALID_ARG, "%s: q_len must be 1 to 65536 (got %u)", who, p.q_len);
+    AK_REQUIRE(p.q_len >= 1 && (uint64_t)p.q_len * p.heads <= (1u << 24), AK_ERR_INVALID_ARG, "%s: q_len (%u) must be positive, q_len * heads at most 2^24", who,
+               p.q_len);
     AK_REQUIRE(p.max_blocks_per_seq >= 1 && p.max_blocks_per_seq <= (1u << 26), AK_ERR_INVALID_ARG, "%s: max_blocks_per_seq must be 1 to 2^26 (got %u)", who,
                p.max_blocks_per_seq);
     AK_REQUIRE(p.n_splits <= AQ_MAX_SPLITS, AK_ERR_INVALID_ARG, "%s: n_splits must be at most %u (got %u)", who, AQ_MAX_SPLITS, p.n_splits);

@@ -8,6 +8,7 @@ default stream).
 from __future__ import annotations
 
 import ctypes as C
+import sys
 
 from . import (AK_BF16, AK_F32, AkashaError, AttnCachedMeta, AttnDecodeParams, AttnQ8Params, CacheWriteMeta, EmbeddingMeta, FlashAttnMeta,
                HeadMoveMeta, MatMulMeta, NormMeta, RopeMeta, RopeOffsetMeta, SoftmaxRectMeta, check, lib)
@@ -173,38 +174,50 @@ def transpose_to_bf16(w_kn, wt_nk, k, n, stream=None):
 
 
 # ---- 8-bit operators -------------------------------------------------------------------------
-_NAMES = {AK_F32: "torch.float32", AK_BF16: "torch.bfloat16"}
-_F32, _I8, _I32 = "torch.float32", "torch.int8", "torch.int32"
+class _Types:
+    """torch's dtypes, once a tensor has come by (the package itself does not import torch)."""
+    f32 = bf16 = i8 = i32 = None
+    of = {AK_F32: None, AK_BF16: None}      # ak_dtype -> torch dtype
 
 
 def _t(x, name, dtype, n, null=False):
     """The pointer of `x`. A tensor has to be contiguous, of `dtype` and on a GPU, with at least `n` elements: the kernels know pointers and
     sizes only, so anything else would be read as something that it is not. A raw pointer is taken as it is."""
+    if getattr(x, "dtype", 0) is dtype and x.is_cuda and x.numel() >= n and x.is_contiguous():
+        return x.data_ptr()
     if x is None:
         if null:
             return None
         raise AkashaError(100, f"{name} is missing")
     if not hasattr(x, "data_ptr"):
         return int(x)
-    if not x.is_cuda or not x.is_contiguous() or x.numel() < n or str(x.dtype) != dtype:
-        raise AkashaError(100, f"{name} has to be a contiguous {dtype} CUDA tensor of at least {n} elements, got {tuple(x.shape)} {x.dtype} on {x.device} "
-                               f"with strides {tuple(x.stride())}")
-    return x.data_ptr()
+    raise AkashaError(100, f"{name} has to be a contiguous {dtype} CUDA tensor of at least {n} elements, got {tuple(x.shape)} {x.dtype} on {x.device} "
+                           f"with strides {tuple(x.stride())}")
+
+
+def _types():
+    if _Types.f32 is None and "torch" in sys.modules:
+        torch = sys.modules["torch"]
+        _Types.of = {AK_F32: torch.float32, AK_BF16: torch.bfloat16}
+        _Types.bf16, _Types.i8, _Types.i32, _Types.f32 = torch.bfloat16, torch.int8, torch.int32, torch.float32
+    return _Types
 
 
 def rmsnorm_q8(x, residual, weight, q, scales, rows, size, eps=1e-5, in_dtype=AK_F32, stream=None):
     """RMS norm of `rows` rows of `size` values, with `residual` added first (and written back to `x`) where it is given, as int8 `q` with one
     f32 scale per row. `weight=None`: no norm, the rows are quantised as they are."""
+    y = _types()
     n = rows * size
-    check(lib().ak_rmsnorm_q8(_s(stream), _t(x, "x", _NAMES.get(in_dtype), n), in_dtype, _t(residual, "residual", _F32, n, True),
-                              _t(weight, "weight", _F32, size, True), _t(q, "q", _I8, n), _t(scales, "scales", _F32, rows), NormMeta(rows, size, eps)))
+    check(lib().ak_rmsnorm_q8(_s(stream), _t(x, "x", y.of.get(in_dtype), n), in_dtype, _t(residual, "residual", y.f32, n, True),
+                              _t(weight, "weight", y.f32, size, True), _t(q, "q", y.i8, n), _t(scales, "scales", y.f32, rows), NormMeta(rows, size, eps)))
 
 
 def gemm_q8(a, a_scales, wt, w_scales, c, m, n, k, epilogue=0, stream=None, ldc=0):
     """C[m,n] (op)= (A[m,k] @ Wt[n,k]^T) * a_scales[m] * w_scales[n], A and Wt int8, sums exact; `ldc` = row pitch of C in elements (0 = n)."""
+    y = _types()
     ld = ldc or n
-    check(lib().ak_gemm_q8(_s(stream), _t(a, "a", _I8, m * k), _t(a_scales, "a_scales", _F32, m), _t(wt, "wt", _I8, n * k),
-                           _t(w_scales, "w_scales", _F32, n), _t(c, "c", _F32 if epilogue < 2 else "torch.bfloat16", (m - 1) * ld + n if m else 0),
+    check(lib().ak_gemm_q8(_s(stream), _t(a, "a", y.i8, m * k), _t(a_scales, "a_scales", y.f32, m), _t(wt, "wt", y.i8, n * k),
+                           _t(w_scales, "w_scales", y.f32, n), _t(c, "c", y.f32 if epilogue < 2 else y.bf16, (m - 1) * ld + n if m else 0),
                            MatMulMeta(m, n, k), epilogue, ld))
 
 
@@ -212,30 +225,33 @@ def rope_kv_append_q8(qkv, rope_table, rope_len, positions, slots, q_out, k_pool
                       pool_blocks, dtype=AK_BF16, stream=None):
     """Head split, RoPE and append to the 8-bit cache: the rotated queries go to `q_out` (`dtype`), keys and values to int8 rows of their slot
     with one scale per (slot, kv head). No two tokens of a call may have the same slot."""
+    y = _types()
     pool = pool_blocks * kv_heads * 16
     check(lib().ak_rope_kv_append_q8(
-        _s(stream), _t(qkv, "qkv", _F32, tokens * (heads + 2 * kv_heads) * head_dim), _t(rope_table, "rope_table", _F32, rope_len * head_dim), rope_len,
-        _t(positions, "positions", _I32, tokens), _t(slots, "slots", _I32, tokens), _t(q_out, "q_out", _NAMES.get(dtype), tokens * heads * head_dim),
-        _t(k_pool, "k_pool", _I8, pool * head_dim), _t(v_pool, "v_pool", _I8, pool * head_dim), _t(k_scales, "k_scales", _F32, pool),
-        _t(v_scales, "v_scales", _F32, pool), tokens, heads, kv_heads, head_dim, 16, dtype, pool_blocks))
+        _s(stream), _t(qkv, "qkv", y.f32, tokens * (heads + 2 * kv_heads) * head_dim), _t(rope_table, "rope_table", y.f32, rope_len * head_dim), rope_len,
+        _t(positions, "positions", y.i32, tokens), _t(slots, "slots", y.i32, tokens), _t(q_out, "q_out", y.of.get(dtype), tokens * heads * head_dim),
+        _t(k_pool, "k_pool", y.i8, pool * head_dim), _t(v_pool, "v_pool", y.i8, pool * head_dim), _t(k_scales, "k_scales", y.f32, pool),
+        _t(v_scales, "v_scales", y.f32, pool), tokens, heads, kv_heads, head_dim, 16, dtype, pool_blocks))
 
 
 def kv_read_q8(k_pool, v_pool, k_scales, v_scales, slots, k_out, v_out, tokens, kv_heads, head_dim, pool_blocks, dtype=AK_BF16, stream=None):
     """Rows of the 8-bit cache as numbers: `k_out`, `v_out` [tokens, kv_heads * head_dim] (`dtype`, either may be None) of the given slots."""
+    y = _types()
     pool, n = pool_blocks * kv_heads * 16, tokens * kv_heads * head_dim
     check(lib().ak_kv_read_q8(
-        _s(stream), _t(k_pool, "k_pool", _I8, pool * head_dim), _t(v_pool, "v_pool", _I8, pool * head_dim), _t(k_scales, "k_scales", _F32, pool),
-        _t(v_scales, "v_scales", _F32, pool), _t(slots, "slots", _I32, tokens), _t(k_out, "k_out", _NAMES.get(dtype), n, True),
-        _t(v_out, "v_out", _NAMES.get(dtype), n, True), tokens, kv_heads, head_dim, 16, dtype, pool_blocks))
+        _s(stream), _t(k_pool, "k_pool", y.i8, pool * head_dim), _t(v_pool, "v_pool", y.i8, pool * head_dim), _t(k_scales, "k_scales", y.f32, pool),
+        _t(v_scales, "v_scales", y.f32, pool), _t(slots, "slots", y.i32, tokens), _t(k_out, "k_out", y.of.get(dtype), n, True),
+        _t(v_out, "v_out", y.of.get(dtype), n, True), tokens, kv_heads, head_dim, 16, dtype, pool_blocks))
 
 
 def attn_decode_paged_q8(q, k_pool, v_pool, k_scales, v_scales, block_tables, kv_lens, out, rows, q_len, heads, kv_heads, head_dim, max_blocks_per_seq, scale,
                          pool_blocks, dtype=AK_BF16, n_splits=0, stream=None):
     """Attention of the newest `q_len` tokens of every sequence over the 8-bit cache, each seeing the positions up to its own (`kv_lens` counts
     the new tokens). Needs no scratch."""
+    y = _types()
     pool, n = pool_blocks * kv_heads * 16, rows * q_len * heads * head_dim
     check(lib().ak_attn_decode_paged_q8(
-        _s(stream), _t(q, "q", _NAMES.get(dtype), n), _t(k_pool, "k_pool", _I8, pool * head_dim), _t(v_pool, "v_pool", _I8, pool * head_dim),
-        _t(k_scales, "k_scales", _F32, pool), _t(v_scales, "v_scales", _F32, pool), _t(block_tables, "block_tables", _I32, rows * max_blocks_per_seq),
-        _t(kv_lens, "kv_lens", _I32, rows), _t(out, "out", _NAMES.get(dtype), n),
+        _s(stream), _t(q, "q", y.of.get(dtype), n), _t(k_pool, "k_pool", y.i8, pool * head_dim), _t(v_pool, "v_pool", y.i8, pool * head_dim),
+        _t(k_scales, "k_scales", y.f32, pool), _t(v_scales, "v_scales", y.f32, pool), _t(block_tables, "block_tables", y.i32, rows * max_blocks_per_seq),
+        _t(kv_lens, "kv_lens", y.i32, rows), _t(out, "out", y.of.get(dtype), n),
         AttnQ8Params(rows, q_len, heads, kv_heads, head_dim, 16, max_blocks_per_seq, scale, dtype, n_splits, pool_blocks)))

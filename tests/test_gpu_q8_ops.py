@@ -186,6 +186,20 @@ def test_gemm_rows_do_not_depend_on_the_batch(ak, torch_cuda):
         assert torch.equal(c, full[:m]), m
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 100, 64), (64, 2048, 4096), (1300, 520, 256)])
+def test_gemm_scales_at_any_alignment(ak, torch_cuda, m, n, k):
+    """Scales that begin at an odd element: the same bits."""
+    torch = torch_cuda
+    g = _gen(torch, 6)
+    a, wt = _int8(torch, (m, k), g), _int8(torch, (n, k), g)
+    sa, sw = torch.rand(m + 1, device="cuda", generator=g), torch.rand(n + 1, device="cuda", generator=g)
+    c, want = torch.empty(m, n, device="cuda"), torch.empty(m, n, device="cuda")
+    ak.ops.gemm_q8(a, sa[1:], wt, sw[1:], c, m, n, k)
+    ak.ops.gemm_q8(a, sa[1:].clone(), wt, sw[1:].clone(), want, m, n, k)
+    torch.cuda.synchronize()
+    assert torch.equal(c, want)
+
+
 @pytest.mark.parametrize("m", [3, 1100])
 def test_gemm_passes_scales_that_are_not_finite_on(ak, torch_cuda, m):
     torch = torch_cuda
@@ -475,8 +489,21 @@ def test_attn_far_blocks(ak, torch_cuda):
 
 # ------------------------------------------------------------------ streams, graphs
 def _work(ak, torch, seed):
-    """One call of every operator on buffers of its own: (call(stream), the outputs)."""
+    """One call of every operator on buffers of its own: (call(stream), the outputs). Odd seeds: a decode step of 40 sequences; even ones: long
+    sequences that are split, and a product of many rows."""
     g = _gen(torch, seed)
+    if seed % 2 == 0:
+        x, w = torch.randn(2048, 768, device="cuda", generator=g), torch.rand(768, device="cuda", generator=g)
+        q8, s8 = torch.empty(2048, 768, dtype=torch.int8, device="cuda"), torch.empty(2048, device="cuda")
+        wt, sw = _int8(torch, (1536, 768), g), torch.rand(1536, device="cuda", generator=g)
+        y, out = torch.empty(2048, 1536, device="cuda"), torch.empty(2, 768, device="cuda")
+        cache, tables, klens, blocks, mb = _attn_case(torch, [5000, 4099], 12, 64, seed)
+
+        def long_call(stream):
+            ak.ops.rmsnorm_q8(x, None, w, q8, s8, 2048, 768, stream=stream)
+            ak.ops.gemm_q8(q8, s8, wt, sw, y, 2048, 1536, 768, stream=stream)
+            ak.ops.attn_decode_paged_q8(x, *cache, tables, klens, out, 2, 1, 12, 12, 64, mb, 0.125, blocks, dtype=ak.AK_F32, stream=stream)
+        return long_call, [q8, s8, y, out], x
     x, w = torch.randn(40, 768, device="cuda", generator=g), torch.rand(768, device="cuda", generator=g)
     q8, s8 = torch.empty(40, 768, dtype=torch.int8, device="cuda"), torch.empty(40, device="cuda")
     wt, sw = _int8(torch, (2304, 768), g), torch.rand(2304, device="cuda", generator=g)
@@ -528,7 +555,7 @@ def test_captured_and_replayed_on_new_inputs(ak, torch_cuda):
         with torch.cuda.graph(graph):
             call(torch.cuda.current_stream().cuda_stream)
         graphs.append(graph)
-    fresh = [torch.randn(40, 768, device="cuda", generator=_gen(torch, 8 + i)) for i in range(2)]
+    fresh = [torch.randn(x.shape, device="cuda", generator=_gen(torch, 8 + i)) for i, (_, _, x) in enumerate(works)]
     want = []
     for (call, outs, x), f in zip(works, fresh):
         x.copy_(f)

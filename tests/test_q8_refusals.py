@@ -38,7 +38,7 @@ CACHE = [("k_pool", P + 8), ("v_scales", P + 4), ("kv_heads", 0), ("kv_heads", 3
                     ("kv_read_q8", READ, b) for b in [{k: v} for k, v in CACHE if k != "heads" and (k, v) != ("kv_heads", 3)] + [
                         dict(k_out=None, v_out=None), dict(slots=0), dict(k_out=P + 8), dict(v_out=P + 4), dict(slots=P + 1)]] + [
                             ("attn_decode_paged_q8", ATTN, {k: v}) for k, v in CACHE + [
-                                ("q", 0), ("out", 0), ("block_tables", 0), ("kv_lens", 0), ("q_len", 0), ("q_len", 65537), ("n_splits", 17), ("max_blocks_per_seq", 0),
+                                ("q", 0), ("out", 0), ("block_tables", 0), ("kv_lens", 0), ("q_len", 0), ("q_len", (1 << 22) + 1), ("q_len", (1 << 32) - 1), ("n_splits", 17), ("max_blocks_per_seq", 0),
                                 ("max_blocks_per_seq", (1 << 26) + 1), ("q", P + 8), ("out", P + 2), ("kv_lens", P + 2)]])
 def test_refused(ak, name, good, bad):
     e = _call(ak, name, good, **bad)
