@@ -22,8 +22,8 @@
 // reduction over the lanes stands between the two products.
 //
 // Measured (graph of launches on three sets of inputs, cold L2): 64 sequences x 16 heads x 128, 64 to 4096 positions 90 us = 0.96 of the copy
-// bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 24 us = 0.68: bound by instructions there (231 a tile of 2176 bytes, issue
-// slots 72 % busy); 2 sequences of 60000 x 8 kv heads x 16 query rows 63 us = 0.59: few CTAs, instructions; one sequence of 300 x 5 heads
+// bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 22.6 us = 0.73: bound by instructions there (some 210 a tile of 2176 bytes, issue
+// slots three quarters busy); 2 sequences of 60000 x 8 kv heads x 16 query rows 63 us = 0.59: few CTAs, instructions; one sequence of 300 x 5 heads
 // 5.8 us, a chain of latencies (an empty launch takes 2).
 //
 // A CTA takes one (sequence, kv head, tile of queries, split); each warp has every n-th cache block of the split and a ring of cp.async
@@ -178,6 +178,9 @@ __global__ void __launch_bounds__(AQ_MAX_WARPS * 32, AqCfg<HD>::CTAS)
 attn_decode_q8_kernel(const AqArgs a) {
     using C = AqCfg<HD>;
     constexpr int STAGES = C::STAGES;
+    // Tiles of a turn of the loop: two share its votes, waits and addresses where the registers allow it (64 x 12 heads x 64 x 1024, f32 24.4 -> 22.6 us,
+    // 128 x 5 heads x 32 36.8 -> 33.9; at head size 128 four stages leave room for 12 warps on an SM: 90 -> 101 us).
+    constexpr int TURN = HD == 128 || (HD == 64 && NQ == 2) ? 1 : 2;
     constexpr int ROWS = 4 * NQ;                     // queries of a tile: NQ column blocks of 4
     constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;   // of a query
     constexpr int KW = HD / 16, KS = HD / 32;        // words of a key row per lane, steps of K q
@@ -279,7 +282,7 @@ attn_decode_q8_kernel(const AqArgs a) {
         cp_commit();
     };
 #pragma unroll
-    for (uint32_t i = 0; i + 1 < (uint32_t)STAGES; i++) request();
+    for (int i = 0; i < STAGES - TURN; i++) request();
 
     // ---- queries: digits into shared memory, for every warp
     for (uint32_t i = threadIdx.x; i < ROWS * 8; i += blockDim.x) {   // whole groups of 8: blockDim.x and ROWS * 8 are multiples of 32
@@ -327,7 +330,8 @@ attn_decode_q8_kernel(const AqArgs a) {
     }
     __syncthreads();
     // operand lane (g, t): column g = digit g & 1 of query g >> 1 of each block (3 digits: of a second block, digits 2 and the zeros)
-    uint32_t qb[NQ][KS][DIGITS == 3 ? 4 : 2];
+    constexpr int QK = DIGITS == 3 ? 2 : 1;
+    uint32_t qb[NQ][KS][2 * QK];
     float row_scale[NQ];
 #pragma unroll
     for (int u = 0; u < NQ; u++) {
@@ -356,110 +360,144 @@ attn_decode_q8_kernel(const AqArgs a) {
         for (int j = 0; j < MT; j++) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.0f;
     int v_exp = -110;   // weights are p * vs * 2^(5 - v_exp) with vs < 2^v_exp for every finite value scale so far
 
-    for (uint32_t i = 0; i < mine; i++) {
-        request();
-        cp_wait<STAGES - 1>();
+    for (uint32_t i = 0; i < mine; i += TURN) {
+#pragma unroll
+        for (int b = 0; b < TURN; b++) request();
+        cp_wait<STAGES - TURN>();
         __syncwarp();
-        if (there & (1u << (STAGES - 1))) {
-            const uint32_t ksm = get, vsm = get + C::TILE, sks = get + 2 * C::TILE + 4 * g;
-            // ---- S^T = K q: positions g, g + 8 of query t
-            int32_t dot[NQ][DIGITS == 3 ? 2 : 1][4];
-            {
-                uint32_t k0[KW], k1[KW];
-                at_lane.load_key(ksm, k0);
-                at_lane.load_key(ksm + 8 * HD, k1);
+        uint32_t tile[TURN];    // where the turn's tiles are
+        int32_t pos[TURN];      // this lane's first position of each (its second is 8 further); none that anybody sees for a tile that is not there
 #pragma unroll
-                for (int k = 0; k < KS; k++)
+        for (int b = 0; b < TURN; b++) {
+            tile[b] = get;
+            get = get == ring + (STAGES - 1) * C::STAGE ? ring : get + C::STAGE;
+            pos[b] = (there >> (STAGES - 1 - b)) & 1u ? pos0 + (int32_t)g : 1 << 30;
+            pos0 += (int32_t)(warps * Q8_BS);
+        }
+        // every row sees all of every tile
+        const bool whole = pos0 + (int32_t)(Q8_BS - warps * Q8_BS) <= lim_min && ((there >> (STAGES - TURN)) & ((1u << TURN) - 1)) == (1u << TURN) - 1;
+        // ---- S^T = K q: positions g, g + 8 of query t
+        int32_t dot[TURN][NQ][QK][4];
+        float ks[TURN][2], vs[TURN][2];
 #pragma unroll
-                    for (int u = 0; u < NQ; u++) {
+        for (int b = 0; b < TURN; b++) {
+            uint32_t k0[KW], k1[KW];
+            at_lane.load_key(tile[b], k0);
+            at_lane.load_key(tile[b] + 8 * HD, k1);
 #pragma unroll
-                        for (int d = 0; d < (DIGITS == 3 ? 2 : 1); d++) {
-                            if (k == 0) mma_s8_first(dot[u][d], k0[0], k1[0], k0[1], k1[1], qb[u][0][2 * d], qb[u][0][2 * d + 1]);
-                            else mma_s8(dot[u][d], k0[2 * k], k1[2 * k], k0[2 * k + 1], k1[2 * k + 1], qb[u][k][2 * d], qb[u][k][2 * d + 1]);
-                        }
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int u = 0; u < NQ; u++)
+#pragma unroll
+                    for (int d = 0; d < QK; d++) {
+                        if (k == 0) mma_s8_first(dot[b][u][d], k0[0], k1[0], k0[1], k1[1], qb[u][0][2 * d], qb[u][0][2 * d + 1]);
+                        else mma_s8(dot[b][u][d], k0[2 * k], k1[2 * k], k0[2 * k + 1], k1[2 * k + 1], qb[u][k][2 * d], qb[u][k][2 * d + 1]);
                     }
-            }
-            const float ka = lds_f(sks), kb = lds_f(sks + 32), va = lds_f(sks + 64), vb = lds_f(sks + 96);
-            const bool whole = pos0 + (int32_t)Q8_BS <= lim_min;   // every row sees the whole tile
-            float x[NQ][2], p[NQ][2], most = -INFINITY;   // q . k without scales; exponents 2^..; the largest of these
+            const uint32_t sks = tile[b] + 2 * C::TILE + 4 * g;
+            ks[b][0] = lds_f(sks); ks[b][1] = lds_f(sks + 32);
+            vs[b][0] = lds_f(sks + 64); vs[b][1] = lds_f(sks + 96);
+        }
+        float x[TURN][NQ][2], p[TURN][NQ][2], most = -INFINITY, v_most = 0.0f;   // q . k without scales; exponents 2^..; the largest of these; of the value scales
+#pragma unroll
+        for (int b = 0; b < TURN; b++) {
+            v_most = fmaxf(v_most, fmaxf(fabsf(vs[b][0]), fabsf(vs[b][1])));
+#pragma unroll
+            for (int u = 0; u < NQ; u++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int32_t two = dot[b][u][0][2 * h] * 256 + dot[b][u][0][2 * h + 1];
+                    x[b][u][h] = QK == 2 ? fmaf((float)two, 256.0f, (float)dot[b][u][QK - 1][2 * h]) : (float)two;
+                    // (a row without a reference yet has +infinity here for every score)
+                    p[b][u][h] = fmaf(x[b][u][h], row_scale[u] * ks[b][h], -m_ref[u]);
+                    most = fmaxf(most, p[b][u][h]);
+                }
+        }
+        // A score more than 8 above its row's reference, or a value scale that the weights' power of two does not cover yet. (In a turn that not every
+        // row sees to its end, also by what nobody sees: the branch looks again.)
+        if (__any_sync(0xffffffffu, most > 8.0f || v_most >= pow2i(v_exp))) {
+            float vtop = 0.0f;
+#pragma unroll
+            for (int b = 0; b < TURN; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (pos[b] + 8 * h < lim_max && fabsf(vs[b][h]) < INFINITY) vtop = fmaxf(vtop, fabsf(vs[b][h]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
+            const int ve = (int)(__float_as_uint(vtop) >> 23) - 126;   // vtop < 2^ve
+            float regrade = 1.0f;
+            if (ve > v_exp) { regrade = ve - v_exp > 120 ? 0.0f : pow2i(v_exp - ve); v_exp = ve; }   // the same in every lane
+            float corr[NQ];
 #pragma unroll
             for (int u = 0; u < NQ; u++) {
-                if constexpr (DIGITS == 3) {
-                    x[u][0] = fmaf((float)(dot[u][0][0] * 256 + dot[u][0][1]), 256.0f, (float)dot[u][1][0]);
-                    x[u][1] = fmaf((float)(dot[u][0][2] * 256 + dot[u][0][3]), 256.0f, (float)dot[u][1][2]);
-                } else {
-                    x[u][0] = (float)(dot[u][0][0] * 256 + dot[u][0][1]);
-                    x[u][1] = (float)(dot[u][0][2] * 256 + dot[u][0][3]);
-                }
-                // (a row without a reference yet has +infinity here for every score)
-                p[u][0] = fmaf(x[u][0], row_scale[u] * ka, -m_ref[u]);
-                p[u][1] = fmaf(x[u][1], row_scale[u] * kb, -m_ref[u]);
-                most = fmaxf(most, fmaxf(p[u][0], p[u][1]));
-            }
-            // A score more than 8 above its row's reference, or a value scale that the weights' power of two does not cover yet. (In a tile that not
-            // every row sees to its end, also by what nobody sees: the branch looks again.)
-            if (__any_sync(0xffffffffu, most > 8.0f || fmaxf(fabsf(va), fabsf(vb)) >= pow2i(v_exp))) {
-                const int32_t pa = pos0 + (int32_t)g, pb = pa + 8;
-                float vtop = fmaxf(fabsf(va) < INFINITY && pa < lim_max ? fabsf(va) : 0.0f, fabsf(vb) < INFINITY && pb < lim_max ? fabsf(vb) : 0.0f);
+                float mb = -INFINITY;
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
-                const int ve = (int)(__float_as_uint(vtop) >> 23) - 126;   // vtop < 2^ve
-                float regrade = 1.0f;
-                if (ve > v_exp) { regrade = ve - v_exp > 120 ? 0.0f : pow2i(v_exp - ve); v_exp = ve; }   // the same in every lane
-                float corr[NQ];
+                for (int b = 0; b < TURN; b++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        p[b][u][h] = x[b][u][h] * (row_scale[u] * ks[b][h]);
+                        if (pos[b] + 8 * h < lim[u]) mb = fmaxf(mb, p[b][u][h]);
+                    }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+                const float m_new = fmaxf(m_ref[u], mb);
+                corr[u] = m_new == -INFINITY ? 1.0f : ex2(m_ref[u] - m_new);
+                m_ref[u] = m_new;
+#pragma unroll
+                for (int b = 0; b < TURN; b++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) p[b][u][h] -= m_new;
+                l_run[u] *= corr[u];
+                corr[u] *= regrade;
+            }
+#pragma unroll
+            for (int u = 0; u < NP; u++) {
+                const float c0 = TWO ? corr[u] : corr[(2 * u) % NQ], c1 = TWO ? corr[u] : corr[(2 * u + 1) % NQ];
+#pragma unroll
+                for (int j = 0; j < MT; j++) { acc[u][j][0] *= c0; acc[u][j][1] *= c1; acc[u][j][2] *= c0; acc[u][j][3] *= c1; }
+            }
+        }
+        const float vf = pow2i(5 - v_exp);
+        float w[TURN][NQ][2];
+#pragma unroll
+        for (int b = 0; b < TURN; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float f = vs[b][h] * vf;
 #pragma unroll
                 for (int u = 0; u < NQ; u++) {
-                    const float s0 = x[u][0] * (row_scale[u] * ka), s1 = x[u][1] * (row_scale[u] * kb);
-                    float mb = fmaxf(pa < lim[u] ? s0 : -INFINITY, pb < lim[u] ? s1 : -INFINITY);
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
-                    const float m_new = fmaxf(m_ref[u], mb);
-                    corr[u] = m_new == -INFINITY ? 1.0f : ex2(m_ref[u] - m_new);
-                    m_ref[u] = m_new;
-                    p[u][0] = s0 - m_new;
-                    p[u][1] = s1 - m_new;
-                    l_run[u] *= corr[u];
-                    corr[u] *= regrade;
-                }
-#pragma unroll
-                for (int u = 0; u < NP; u++) {
-                    const float c0 = TWO ? corr[u] : corr[(2 * u) % NQ], c1 = TWO ? corr[u] : corr[(2 * u + 1) % NQ];
-#pragma unroll
-                    for (int j = 0; j < MT; j++) { acc[u][j][0] *= c0; acc[u][j][1] *= c1; acc[u][j][2] *= c0; acc[u][j][3] *= c1; }
+                    p[b][u][h] = ex2(p[b][u][h]);
+                    w[b][u][h] = p[b][u][h] * f;
                 }
             }
-            const float vf = pow2i(5 - v_exp), fa = va * vf, fb = vb * vf;
-            float w[NQ][2];
+        if (!whole) {   // positions that a row does not see may hold anything, a NaN for a scale included
 #pragma unroll
-            for (int u = 0; u < NQ; u++) {
-                p[u][0] = ex2(p[u][0]);
-                p[u][1] = ex2(p[u][1]);
-                w[u][0] = p[u][0] * fa;
-                w[u][1] = p[u][1] * fb;
-            }
-            if (!whole) {   // positions that a row does not see may hold anything, a NaN for a scale included
-                const int32_t pa = pos0 + (int32_t)g, pb = pa + 8;
+            for (int b = 0; b < TURN; b++)
 #pragma unroll
-                for (int u = 0; u < NQ; u++) {
-                    if (pa >= lim[u]) p[u][0] = w[u][0] = 0.0f;
-                    if (pb >= lim[u]) p[u][1] = w[u][1] = 0.0f;
-                }
-            }
+                for (int u = 0; u < NQ; u++)
 #pragma unroll
-            for (int u = 0; u < NQ; u++) l_run[u] += p[u][0] + p[u][1];   // this lane's positions only: added up over the lanes at the end
+                    for (int h = 0; h < 2; h++)
+                        if (pos[b] + 8 * h >= lim[u]) p[b][u][h] = w[b][u][h] = 0.0f;
+        }
+#pragma unroll
+        for (int b = 0; b < TURN; b++)
+#pragma unroll
+            for (int u = 0; u < NQ; u++) l_run[u] += p[b][u][0] + p[b][u][1];   // this lane's positions only: added up over the lanes at the end
+#pragma unroll
+        for (int b = 0; b < TURN; b++) {
             uint32_t pw[NP][2];
 #pragma unroll
             for (int u = 0; u < NP; u++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     if constexpr (TWO) {
-                        const float lead = __half2float(__float2half_rn(w[u][h]));
-                        pw[u][h] = transpose8(pack_half2(lead, w[u][h] - lead));
+                        const float lead = __half2float(__float2half_rn(w[b][u][h]));
+                        pw[u][h] = transpose8(pack_half2(lead, w[b][u][h] - lead));
                     } else {
-                        pw[u][h] = transpose8(pack_half2(w[(2 * u) % NQ][h], w[(2 * u + 1) % NQ][h]));
+                        pw[u][h] = transpose8(pack_half2(w[b][(2 * u) % NQ][h], w[b][(2 * u + 1) % NQ][h]));
                     }
                 }
-            // ---- O^T += V p
+            // ---- O^T += V p (a tile that is not there has weights of 0, and int8 is finite whatever its stage holds)
+            const uint32_t vsm = tile[b] + C::TILE;
             uint32_t w0[HD / 32], w1[HD / 32], w2[HD / 32], w3[HD / 32];
             at_lane.load_value(vsm + at_lane.val, w0);
             at_lane.load_value(vsm + at_lane.val2, w1);
@@ -480,8 +518,6 @@ attn_decode_q8_kernel(const AqArgs a) {
                 }
             }
         }
-        get = get == ring + (STAGES - 1) * C::STAGE ? ring : get + C::STAGE;
-        pos0 += (int32_t)(warps * Q8_BS);
         __syncwarp();
     }
     cp_wait<0>();
