@@ -48,6 +48,37 @@ __device__ __forceinline__ void col_scales(const float* w, uint32_t col, uint32_
     }
 }
 
+// One result, with the epilogue's operation; `old` is what it is added to.
+template <int EPI>
+__device__ __forceinline__ void store_one(const GemmEpi& ep, uint32_t row, uint32_t col, float v, float old) {
+    const size_t at = (size_t)row * ep.ldc + col;
+    if constexpr (EPI == AK_EPI_STORE_F32) reinterpret_cast<float*>(ep.c)[at] = v;
+    else if constexpr (EPI == AK_EPI_ADD_F32) reinterpret_cast<float*>(ep.c)[at] = v + old;
+    else reinterpret_cast<bf16*>(ep.c)[at] = __float2bfloat16_rn(EPI == AK_EPI_SILU_BF16 ? epi_silu(v) : v);
+}
+// 16 columns of a warp's 32 rows where rows are not aligned for vectors (an odd pitch, the last columns): turned in shared memory (32 x 17 floats) so
+// that an instruction writes 16 neighbouring elements of two rows instead of one element of 32 (bf16, 6576 x 82 x 256: 11.2 us that way, 4.3 like
+// this; 8000 x 8001 x 1024: 631 and 119, and 64 through TMA with a pitch of 8008). 32 columns at a time, whose rows rotate instead of being padded,
+// cost 6 % more.
+template <int EPI>
+__device__ __forceinline__ void store_rows16(const GemmEpi& ep, float* buf, uint32_t row0, uint32_t m, uint32_t col0, uint32_t n, const float* v, uint32_t lane) {
+    const uint32_t r0 = row0 + (lane >> 4), col = col0 + (lane & 15);
+    float old[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i++) {   // all asked for before the first is needed
+        old[i] = 0.0f;
+        if constexpr (EPI == AK_EPI_ADD_F32)
+            if (r0 + 2 * i < m && col < n) old[i] = reinterpret_cast<const float*>(ep.c)[(size_t)(r0 + 2 * i) * ep.ldc + col];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; j++) buf[lane * 17 + j] = v[j];
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i++)
+        if (r0 + 2 * i < m && col < n) store_one<EPI>(ep, r0 + 2 * i, col, buf[((lane >> 4) + 2 * i) * 17 + (lane & 15)], old[i]);
+}
+
 // ============================================================================ one CTA per tile
 // grid = (n tiles, m tiles, ks), cluster = (1, 1, ks): the CTAs of a cluster take a part of K each, push the column slice that a peer owns
 // into its shared memory, and every one adds up and stores its own slice.
@@ -155,7 +186,9 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
                 for (int j = 0; j < 16; j++) v[j] = (float)(int32_t)r[j] * sa * sw[j];
                 if (c0 + 16 < bn) col_scales<16>(sc.w, n0 + c0 + 16, n, vec, sw);
-                epi_store16<EPI>(ep, row, row < m, n0 + c0, v, n, lane);
+                // (the ring's first 16 KB are free by now: every MMA has read its operands)
+                if (n0 + c0 + 16 <= n && (ep.ldc & 7u) == 0) epi_store16<EPI>(ep, row, row < m, n0 + c0, v, n, lane);
+                else store_rows16<EPI>(ep, reinterpret_cast<float*>(smem) + quad * (32 * 17), m0 + quad * 32, m, n0 + c0, n, v, lane);
             }
         }
     } else {
@@ -186,7 +219,8 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             bool landed = mbar_wait(&xch_bar, 0);
             if (!landed && lane == 0) atomicExch(&fail_flag, 6u);
             got = __all_sync(0xffffffffu, landed);
-            if (got && row < m) {
+            const bool vectors = (ep.ldc & 3u) == 0;
+            if (got && vectors && row < m) {
 #pragma unroll 1
                 for (uint32_t j = 0; j < SL; j += 4) {
                     int4 acc = make_int4(0, 0, 0, 0);
@@ -199,6 +233,22 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     col_scales<4>(sc.w, col, n, vec, s4);
                     const float v[4] = {(float)acc.x * sa * s4[0], (float)acc.y * sa * s4[1], (float)acc.z * sa * s4[2], (float)acc.w * sa * s4[3]};
                     epi_store<EPI, 4>(ep, row, col, v, n);
+                }
+            }
+            if (got && !vectors) {   // an odd pitch: neighbouring lanes take neighbouring columns, of rows that other lanes have put down
+                __syncwarp();
+#pragma unroll 1
+                for (uint32_t i = 0, r = lane / SL, c = lane % SL; i < SL; i++) {
+                    const float s_row = __shfl_sync(0xffffffffu, sa, r & 31u);
+                    const uint32_t col = n0 + rank * SL + c;
+                    const uint32_t row_i = m0 + quad * 32 + r;
+                    if (row_i < m && col < n) {
+                        int32_t acc = 0;
+                        for (uint32_t src = 0; src < ks; src++) acc += red[((size_t)src * a_rows + quad * 32 + r) * SL + c];
+                        const float old = EPI == AK_EPI_ADD_F32 ? reinterpret_cast<const float*>(ep.c)[(size_t)row_i * ep.ldc + col] : 0.0f;
+                        store_one<EPI>(ep, row_i, col, (float)acc * s_row * sc.w[col], old);
+                    }
+                    for (c += 32; c >= SL; c -= SL) r++;
                 }
             }
         }
@@ -361,8 +411,12 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 const uint32_t col = n0 + (OUT_BF16 ? (c0 & ~32u) : c0);   // first column of the staged piece
                 // a store is clipped at n in whole 16-byte units only: a ragged last piece is stored from registers
                 if (!tma_out || (col + CW > n && (n * (OUT_BF16 ? 2u : 4u)) % 16u != 0)) {
+                    if (lane == 0) tma_store_wait_read<0>();   // the staging buffer may still be read by an earlier piece's store
 #pragma unroll
-                    for (int j = 0; j < 32; j += 16) epi_store16<EPI>(ep, row, row < m, n0 + c0 + j, v + j, n, lane);
+                    for (int j = 0; j < 32; j += 16) {
+                        if (n0 + c0 + j + 16 <= n && (ep.ldc & 7u) == 0) epi_store16<EPI>(ep, row, row < m, n0 + c0 + j, v + j, n, lane);
+                        else store_rows16<EPI>(ep, reinterpret_cast<float*>(stage_sm), row0, m, n0 + c0 + j, n, v + j, lane);
+                    }
                     continue;
                 }
                 const bool first_part = !OUT_BF16 || (c0 & 32u) == 0;
@@ -445,13 +499,13 @@ static uint32_t i8_stages(uint32_t bn, uint32_t ks, uint32_t per, uint32_t a_row
 //          from L2; two CTAs on an SM share 121 KB/us, and every further pair of them starts anew. A split adds its exchange.
 //   pair   3.8, and 0.40 per K block of the 74 pairs.
 //   Weights come from HBM at 5.5 MB/us at most.
-static I8Plan i8_plan(uint32_t m, uint32_t n, uint32_t k, bool allow_split) {
+static I8Plan i8_plan(uint32_t m, uint32_t n, uint32_t k) {
     const uint32_t kb = cdiv(k, I8_KB), mt = cdiv(m, I8_M), ar = i8_slot_rows(m);
     const float rows = (float)(m < I8_M ? m : I8_M), stream = (float)n * k / 5.5e6f;
     I8Plan p{};
     float best = 1e30f;
     if (m > I8_M && n > 128) best = 3.8f + (float)cdiv64((uint64_t)cdiv(m, 2 * I8_M) * cdiv(n, I8P_BN), B200_SMS / 2) * kb * 0.40f;
-    for (uint32_t ks = 1; ks <= (allow_split ? 8u : 1u); ks *= 2) {
+    for (uint32_t ks = 1; ks <= 8; ks *= 2) {
         const uint32_t per = cdiv(kb, ks), unit = ks > 4 ? 32 : 16;   // a slice of bn / ks columns is whole groups of 4
         if (ks > 1 && (ks - 1) * per >= kb) break;                    // every CTA of a cluster gets work
         for (uint32_t bn = unit; bn <= 256 && bn < n + 16; bn += bn < 128 ? unit : 32) {
@@ -496,7 +550,7 @@ static int i8_launch_tile(cudaStream_t st, const CUtensorMap& tmA, const CUtenso
 template <int EPI>
 static int i8_launch_epi(cudaStream_t st, const void* a, const void* wt, const GemmEpi& ep, const I8Scales& sc, uint32_t m, uint32_t n, uint32_t k) {
     CUtensorMap tmA, tmB;
-    const I8Plan p = i8_plan(m, n, k, ep.ldc % 4 == 0);
+    const I8Plan p = i8_plan(m, n, k);
     if (!p.bn) {
         static bool set[64] = {};
         AK_TRY(i8_allow_smem(gemm_q8_pair_kernel<EPI>, set, I8_SMEM_PAIR));
