@@ -11,7 +11,7 @@
 //   S^T = K q   m16n8k32 on int8 as it lies in the cache. A query is held as integers X = rint(q F), F = 127 * 256^(D - 1) / max|q|, in
 //               D signed base-256 digits: 2 for bf16 (16 bits of the head's largest value), 3 for f32 (24 bits). Sums of digits are exact.
 //   O^T = V p   m16n8k16 on f16, in which int8 is exact (1024 + 128 + v is put together by a byte permute and 1152 taken off). A weight
-//               w = p vs is its leading f16 part and what is left of it (22 bits together, TWO), or, for bf16 results and more than 4 query
+//               w = p vs is its leading f16 part and what is left of it, times 2^11 (22 bits together, TWO), or, for bf16 results and more than 4 query
 //               rows, the leading part alone (11 bits; the result has 8) with two queries to a column pair.
 // Scores come out with lanes holding positions g, g + 8 of one query, and turn into the second product's operand by a transposition of 8 x 8
 // blocks (movmatrix). With the queries as the 16-row operand of f16 products (and keys converted like values) a tile took 370 instructions and 168
@@ -181,6 +181,7 @@ attn_decode_q8_kernel(const AqArgs a) {
     // Tiles of a turn of the loop: two share its votes, waits and addresses where the registers allow it (64 x 12 heads x 64 x 1024, f32 24.4 -> 22.6 us,
     // 128 x 5 heads x 32 36.8 -> 33.9; at head size 128 four stages leave room for 12 warps on an SM: 90 -> 101 us).
     constexpr int TURN = HD == 128 || (HD == 64 && NQ == 2) ? 1 : 2;
+    constexpr float REST = 2048.0f;                  // what is left of a weight is held times this: at most 2^12, and f16's smallest numbers are of no account
     constexpr int ROWS = 4 * NQ;                     // queries of a tile: NQ column blocks of 4
     constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;   // of a query
     constexpr int KW = HD / 16, KS = HD / 32;        // words of a key row per lane, steps of K q
@@ -491,7 +492,7 @@ attn_decode_q8_kernel(const AqArgs a) {
                 for (int h = 0; h < 2; h++) {
                     if constexpr (TWO) {
                         const float lead = __half2float(__float2half_rn(w[b][u][h]));
-                        pw[u][h] = transpose8(pack_half2(lead, w[b][u][h] - lead));
+                        pw[u][h] = transpose8(pack_half2(lead, (w[b][u][h] - lead) * REST));
                     } else {
                         pw[u][h] = transpose8(pack_half2(w[b][(2 * u) % NQ][h], w[b][(2 * u + 1) % NQ][h]));
                     }
@@ -541,7 +542,7 @@ attn_decode_q8_kernel(const AqArgs a) {
             for (int j = 0; j < MT; j++) {
                 if constexpr (TWO) {
                     *reinterpret_cast<float2*>(wp + (4 * u + t) * HD + 2 * j) =
-                        make_float2((acc[u][j][0] + acc[u][j][1]) * un, (acc[u][j][2] + acc[u][j][3]) * un);
+                        make_float2(fmaf(acc[u][j][1], 1.0f / REST, acc[u][j][0]) * un, fmaf(acc[u][j][3], 1.0f / REST, acc[u][j][2]) * un);
                 } else {
                     *reinterpret_cast<float2*>(wp + (8 * u + t) * HD + 2 * j) = make_float2(acc[u][j][0] * un, acc[u][j][2] * un);
                     *reinterpret_cast<float2*>(wp + (8 * u + 4 + t) * HD + 2 * j) = make_float2(acc[u][j][1] * un, acc[u][j][3] * un);

@@ -137,7 +137,7 @@ norm_q8_kernel(T* __restrict__ x, const float* __restrict__ residual, const floa
 
 // Rows of any size. All the arrays of a row start at the same element offset, so groups are cut where the ADDRESS is a multiple of V elements; the
 // first and last group of a row are partial. With weights (KEEP), resident blocks walk over the rows with a stride that is a multiple of V, so that a block
-// sees one shift only: which of a thread's groups are partial and its weights (in registers) are settled once: 16384 x 2047 45 us, where a
+// sees one shift only: which of a thread's groups are partial and its weights (in registers) are settled once: 16384 x 2047 50 us, where a
 // block per row, its weights put together from two neighbouring vectors, took 56. Without weights there is nothing to keep, and with a
 // residual the loads want blocks coming and going.
 template <typename T, int NV, bool KEEP>
@@ -260,8 +260,8 @@ norm_q8_ragged_kernel(T* __restrict__ x, const float* __restrict__ residual, con
     }
 }
 
-// Rows that do not fit the registers of a block, and buffers that are not aligned for vectors: a block per row, three passes over it (the second and third read what the first wrote back). y is
-// computed twice by the same operations, hence with the same bits.
+// Rows that do not fit the registers of a block, and buffers that are not aligned for vectors: a block per row, three passes over it (the second and
+// third read what the first wrote back). y is computed twice by the same operations, hence with the same bits.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 norm_q8_any_kernel(T* x, const float* residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales, uint32_t size, float eps) {
@@ -560,7 +560,7 @@ int ak_rope_kv_append_q8(void* stream, const float* qkv, const float* rope_table
     const char* who = "ak_rope_kv_append_q8";
     AK_REQUIRE(qkv && rope_table && positions && slots && q_out, AK_ERR_INVALID_ARG, "%s: null pointer", who);
     AK_TRY(q8_check_cache(who, k_pool, v_pool, k_scales, v_scales, heads, kv_heads, head_dim, block_size, q_dtype, pool_blocks));
-    AK_REQUIRE(rope_len >= 1, AK_ERR_INVALID_ARG, "%s: the RoPE table is empty", who);
+    AK_REQUIRE(rope_len >= 1 && rope_len <= 0x7fffffffu, AK_ERR_INVALID_ARG, "%s: the RoPE table must have 1 to 2^31 - 1 positions (got %u)", who, rope_len);
     AK_REQUIRE(q8_aligned(qkv, 16) && q8_aligned(rope_table, 16) && q8_aligned(q_out, 16) && q8_aligned(positions, 4) && q8_aligned(slots, 4),
                AK_ERR_INVALID_ARG, "%s: qkv, q_out and the RoPE table must be 16-byte aligned, positions and slots 4-byte", who);
     AK_REQUIRE(tokens <= 0x7fffffffu, AK_ERR_UNSUPPORTED, "%s: %u tokens are too many for one call", who, tokens);

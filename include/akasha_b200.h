@@ -283,13 +283,14 @@ AK_API int ak_bf16_to_f32(void* stream, const void* src, float* dst, uint64_t n)
 /* RMS norm with the residual's addition and an 8-bit result:
  *   h = x + residual (residual != NULL: f32 x only; h is written back to x), y = h * rsqrt(mean(h^2) + eps) * w per row, q and scales as above.
  *   w == NULL: y = h, the rows are quantised as they are (weights [n,k] for ak_gemm_q8, activations behind SiLU or attention).
- * x [seq_len, size] f32 or bf16 (in_dtype); residual f32, w f32 [size]; q int8 [seq_len, size]; scales f32 [seq_len]. Any size; the
- * fast form wants x and residual aligned to 4 elements and q to 4 bytes (any size), the others run element by element. */
+ * x [seq_len, size] f32 or bf16 (in_dtype); residual f32, w f32 [size]; q int8 [seq_len, size]; scales f32 [seq_len]. Any size;
+ * rows of up to 32768 values (sizes that are no multiple of 16 bytes of x: 16376) are read once if x, residual and w are 16-byte aligned and q to the bytes of 16 bytes of x (4, bf16 8),
+ * others run element by element. */
 AK_API int ak_rmsnorm_q8(void* stream, void* x, uint32_t in_dtype, const float* residual, const float* w, int8_t* q, float* scales, ak_norm_meta m);
 
 /* 8-bit tensor-core product: C[m,n] (op)= (sum_k A[m,k] Wt[n,k]) * a_scales[m] * w_scales[n], A and Wt int8 row-major, sums exact in
  * 32-bit integers, one f32 product with each scale, then the epilogue (ak_gemm_epilogue). ldc: row pitch of C in elements (>= n; as for
- * ak_gemm_bf16_ld an odd width wants a padded pitch). k: a multiple of 16, 16 to 131056. A, Wt and C 16-byte aligned. A row's result is the same
+ * ak_gemm_bf16_ld an odd width wants a padded pitch, up to twice as fast). k: a multiple of 16, 16 to 131056. A, Wt and C 16-byte aligned. A row's result is the same
  * however many rows share the call. */
 AK_API int ak_gemm_q8(void* stream, const int8_t* a, const float* a_scales, const int8_t* wt, const float* w_scales, void* c, ak_matmul_meta m,
                       uint32_t epilogue, uint32_t ldc);
@@ -317,8 +318,8 @@ AK_API int ak_kv_read_q8(void* stream, const int8_t* k_pool, const int8_t* v_poo
  *   block id outside the pool are left out. scale multiplies q . k.
  *   n_splits: CTAs that share a sequence, as one thread-block cluster; 0 = the library's choice, else 1 to 16 (rounded down to a power of two).
  * Sums, maxima and softmax weights are f32. A query is held as integers of 24 bits (f32) or 16 bits (bf16) of its head's largest value (one under
- * 1e-30 counts as 0); the weights of V have 22 bits, or, for bf16 with more than 4 query rows per kv head (q_len * heads / kv_heads), 11. A weight below
- * 2^-29 of its sequence's largest weight-times-scale may count as 0. */
+ * 1e-30 counts as 0); the weights of V have 22 bits, or, for bf16 with more than 4 query rows per kv head (q_len * heads / kv_heads), 11. A weight
+ * times its value's scale below 2^-40 (11 bits: 2^-29) of the sequence's largest value scale may count as 0. */
 typedef struct ak_attn_q8_params {
     uint32_t rows, q_len, heads, kv_heads, head_dim, block_size, max_blocks_per_seq;
     float scale;

@@ -424,6 +424,42 @@ def test_attn_value_scales_of_all_sizes(ak, torch_cuda):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n_splits", [1, 2])
+def test_attn_large_value_that_no_query_looks_at(ak, torch_cuda, dtype, n_splits):
+    """A value a million times the others at a position whose weight vanishes."""
+    torch = torch_cuda
+    dt, tdt = _dt(ak, torch, dtype)
+    lens, heads, hd = [40, 300], 3, 64
+    cache, tables, klens, blocks, mb = _attn_case(torch, lens, heads, hd, 5)
+    q = torch.randn(2, heads * hd, device="cuda", generator=_gen(torch, 2)).to(tdt)
+    big = 2.0 ** 20 * float(cache[3].nan_to_num(0.0).max())
+    for r in range(2):
+        b, p = int(tables[r, 1]), 3
+        cache[0][b, :, p] = (-127 * q[r].view(heads, hd).float().sign()).to(torch.int8)
+        cache[2][b, :, p] = 1.0      # scores of -127 * sum |q| / 8, some -800
+        cache[3][b, :, p] = big
+    out = torch.empty_like(q)
+    ak.ops.attn_decode_paged_q8(q, *cache, tables, klens, out, 2, 1, heads, heads, hd, mb, 0.125, blocks, dtype=dt, n_splits=n_splits)
+    torch.cuda.synchronize()
+    kp, vp, ks, vs = (t.double() for t in cache)
+    for r, n in enumerate(lens):
+        pos = torch.arange(n, device="cuda")
+        b, p = tables[r].long()[pos // 16], pos % 16
+        k, v, x = kp[b, :, p] * ks[b, :, p][..., None], vp[b, :, p] * vs[b, :, p][..., None], q[r].view(heads, hd).double()
+        w = torch.softmax(torch.einsum("kd,jkd->kj", x, k) * 0.125, -1)
+        want, mass = torch.einsum("kj,jkd->kd", w, v), torch.einsum("kj,jkd->kd", w, v.abs())
+        # As in _attn_check, of the positions that weigh anything; and for every position half a step of f16's smallest numbers, 2^-25 / 2^11 with the
+        # factor of a weight's rest, in units of at most 2 * 2^-5 of the largest value scale.
+        k = k[pos != 19].abs()
+        size = torch.einsum("kd,jkd->kj", x.abs(), k) * (hd / 16 + 6) * 2.0 ** -22
+        size = 0.125 * (size + x.abs().amax(-1)[:, None] * k.sum(-1).T * 2.0 ** (-24 if dtype == "f32" else -16))
+        rel = 2 * (float(size.max()) + 2.0 ** -21) + (n / 16 + 40) * 2.0 ** -22
+        err = (out[r].view(heads, hd).double() - want).abs()
+        tol = rel * mass + HALF[dtype] * want.abs() + n * 2.0 ** -40 * 127 * big
+        assert (err <= tol).all(), (r, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("q_len", [1, 5])
 def test_attn_blocks_outside_the_pool(ak, torch_cuda, dtype, q_len):
     """Their positions are left out, whole sequences of them give zeros; lengths past the table are cut."""

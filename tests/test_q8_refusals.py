@@ -33,7 +33,7 @@ CACHE = [("k_pool", P + 8), ("v_scales", P + 4), ("kv_heads", 0), ("kv_heads", 3
         dict(a=0), dict(a_scales=0), dict(wt=0), dict(w_scales=0), dict(c=0), dict(k=0), dict(k=8), dict(k=40), dict(k=131072), dict(epilogue=4), dict(ldc=4),
         dict(a=P + 8), dict(wt=P + 1), dict(c=P + 4), dict(a_scales=P + 2), dict(m=65535 * 128 + 1), dict(n=(1 << 30) + 1)]] + [
             ("rope_kv_append_q8", APPEND, {k: v}) for k, v in CACHE + [
-                ("qkv", 0), ("rope_table", 0), ("positions", 0), ("slots", 0), ("q_out", 0), ("rope_len", 0), ("qkv", P + 4), ("rope_table", P + 8), ("q_out", P + 2),
+                ("qkv", 0), ("rope_table", 0), ("positions", 0), ("slots", 0), ("q_out", 0), ("rope_len", 0), ("rope_len", 1 << 31), ("qkv", P + 4), ("rope_table", P + 8), ("q_out", P + 2),
                 ("slots", P + 2)]] + [
                     ("kv_read_q8", READ, b) for b in [{k: v} for k, v in CACHE if k != "heads" and (k, v) != ("kv_heads", 3)] + [
                         dict(k_out=None, v_out=None), dict(slots=0), dict(k_out=P + 8), dict(v_out=P + 4), dict(slots=P + 1)]] + [
