@@ -364,13 +364,19 @@ static int norm_q8(cudaStream_t st, T* x, const float* residual, const float* w,
 }
 
 // ============================================================================ split + RoPE + quantised append
-// qkv row of a token: `heads` query heads, kv_heads key heads, kv_heads value heads. HD / 4 lanes (HD = 96: 24 of 32) take a head: one
-// float4 each, its two pairs rotated, the largest magnitude of the head by shuffles, 4 bytes out. A block takes one token (several, where
-// their heads do not fill it): position, slot and the lane's RoPE factors are read once for all its heads, 4 of which are in flight at a time.
-constexpr uint32_t AP_THREADS = 256, AP_AHEAD = 4;
+// qkv row of a token: `heads` query heads, kv_heads key heads, kv_heads value heads. A few lanes take a head, 16 values each (HD = 96: 12) as four
+// pieces of 4 that lie HD / 4 apart, so that the lanes of a piece read and write neighbouring bytes; the pairs of a piece are rotated, the largest
+// magnitude of the head goes round by shuffles, 4 bytes a piece go out. The (token, head) rows of a block's tokens lie one behind the other in qkv
+// and are dealt out in turns of one row a group of lanes.
+//
+// With 4 values a lane the hundred instructions that a row takes besides its bytes (addresses, scale, shuffles) were the bound: 16001 tokens, bf16, 12 + 2 x
+// 12 heads of 64 58 us then, 35 now (0.86 of the copy bandwidth); 5 + 2 x 5 of 64, f32 49 and 20; 32 + 2 x 8 of 128 97 and 84 (1.02, 8 pieces
+// 95); 64 tokens of 12 + 2 x 12 heads of 64 2.0 and 1.7.
+constexpr uint32_t AP_THREADS = 256;
 template <int HD> struct ApCfg {
-    static constexpr uint32_t LANES = HD / 4, GROUP = HD == 96 ? 32 : LANES;   // lanes at work / set aside for a head
-    static constexpr uint32_t GROUPS = AP_THREADS / GROUP;
+    static constexpr uint32_t PIECES = HD == 96 ? 3 : 4;       // of four values that a lane holds of a head
+    static constexpr uint32_t LANES = HD / (4 * PIECES);       // of a head
+    static constexpr uint32_t GROUPS = AP_THREADS / LANES;     // rows of a turn
 };
 
 template <typename T, int HD>
@@ -378,67 +384,70 @@ __global__ void __launch_bounds__(AP_THREADS)
 rope_kv_append_q8_kernel(const float* __restrict__ qkv, const float4* __restrict__ rope, uint32_t rope_len, const int32_t* __restrict__ positions,
                          const int32_t* __restrict__ slots, T* __restrict__ q_out, int8_t* __restrict__ k_pool, int8_t* __restrict__ v_pool,
                          float* __restrict__ k_scales, float* __restrict__ v_scales, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t pool_slots,
-                         uint32_t per_block) {
+                         uint32_t per_block, const Q8Div total) {
     using C = ApCfg<HD>;
+    constexpr uint32_t P = C::PIECES, STEP = 4 * C::LANES;   // values between a lane's pieces
     pdl_wait();
     pdl_trigger();
-    const uint32_t total = heads + 2 * kv_heads, group = threadIdx.x / C::GROUP, l = threadIdx.x % C::GROUP;
-    const uint32_t mine = per_block > 1 ? group / total : 0;   // which of the block's tokens
-    const uint32_t t = blockIdx.x * per_block + mine;
-    uint32_t h = per_block > 1 ? group - mine * total : group;
-    const bool on = t < tokens && mine < per_block && l < C::LANES;
-    int32_t pos = -1, slot = -1;
-    if (on) { pos = positions[t]; slot = slots[t]; }
-    const bool live = on && (uint32_t)pos < rope_len;   // a token at another position is left out
-    const float* row = qkv + ((uint64_t)(live ? t : 0) * total) * HD + 4 * (l < C::LANES ? l : 0);
-    float4 f = make_float4(1.f, 0.f, 1.f, 0.f);
-    if (live) f = rope[(uint64_t)pos * (HD / 4) + l];   // (cos, sin) of pairs 2l and 2l + 1
-    const uint64_t block = (uint32_t)slot / Q8_BS, place = (uint32_t)slot % Q8_BS;
-    const bool cached = (uint32_t)slot < pool_slots;
+    const uint32_t group = threadIdx.x / C::LANES, l = threadIdx.x % C::LANES;
+    const uint32_t t0 = blockIdx.x * per_block, items = min(per_block, tokens - t0) * total.d;
+    const float* rows = qkv + (uint64_t)t0 * total.d * HD + 4 * l;
     // whole blocks go round together: the shuffles want every lane of a group
-    for (uint32_t base = 0; base < total; base += AP_AHEAD * C::GROUPS) {
-        float4 x[AP_AHEAD];
+    for (uint32_t base = 0; base < items; base += C::GROUPS) {
+        const uint32_t i = base + group, of_block = total.of(i), tok = t0 + of_block, head = i - of_block * total.d;
+        float4 x[P];
+        int32_t pos = -1, slot = -1;
 #pragma unroll
-        for (uint32_t j = 0; j < AP_AHEAD; j++) {
-            x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (live && h + j * C::GROUPS < total) x[j] = *reinterpret_cast<const float4*>(row + (uint64_t)(h + j * C::GROUPS) * HD);
+        for (uint32_t c = 0; c < P; c++) x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < items) {
+#pragma unroll
+            for (uint32_t c = 0; c < P; c++) x[c] = *reinterpret_cast<const float4*>(rows + (uint64_t)i * HD + c * STEP);
+            pos = positions[tok];
+            if (head >= heads) slot = slots[tok];
         }
+        const bool live = (uint32_t)pos < rope_len;   // a token at another position is left out
+        float4 f[P];   // (cos, sin) of the pieces' pairs
 #pragma unroll
-        for (uint32_t j = 0; j < AP_AHEAD; j++) {
-            const uint32_t hj = h + j * C::GROUPS;
-            if (hj < heads + kv_heads) {
-                rope_rotate(x[j].x, x[j].y, f.x, f.y, x[j].x, x[j].y);
-                rope_rotate(x[j].z, x[j].w, f.z, f.w, x[j].z, x[j].w);
+        for (uint32_t c = 0; c < P; c++) {
+            f[c] = make_float4(1.f, 0.f, 1.f, 0.f);
+            if (live && head < heads + kv_heads) f[c] = rope[(uint64_t)pos * (HD / 4) + c * C::LANES + l];
+        }
+        if (head < heads + kv_heads) {
+#pragma unroll
+            for (uint32_t c = 0; c < P; c++) {
+                rope_rotate(x[c].x, x[c].y, f[c].x, f[c].y, x[c].x, x[c].y);
+                rope_rotate(x[c].z, x[c].w, f[c].z, f[c].w, x[c].z, x[c].w);
             }
-            if (hj < heads && live) {
-                T* dst = q_out + ((uint64_t)t * heads + hj) * HD + 4 * l;
+        }
+        if (live && head < heads) {
+            T* dst = q_out + ((uint64_t)tok * heads + head) * HD + 4 * l;
+#pragma unroll
+            for (uint32_t c = 0; c < P; c++) {
                 if constexpr (sizeof(T) == 4) {
-                    *reinterpret_cast<float4*>(dst) = x[j];
+                    *reinterpret_cast<float4*>(dst + c * STEP) = x[c];
                 } else {
-                    const bf162 a = __floats2bfloat162_rn(x[j].x, x[j].y), b = __floats2bfloat162_rn(x[j].z, x[j].w);
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+                    const bf162 a = __floats2bfloat162_rn(x[c].x, x[c].y), b = __floats2bfloat162_rn(x[c].z, x[c].w);
+                    *reinterpret_cast<uint2*>(dst + c * STEP) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
                 }
             }
-            const bool kv = hj >= heads && hj < total;
-            if (!__any_sync(0xffffffffu, kv)) continue;   // a warp of query heads
-            uint32_t top = max(max(abs_bits(x[j].x), abs_bits(x[j].y)), max(abs_bits(x[j].z), abs_bits(x[j].w)));
-            if constexpr (C::GROUP == 32) {
-                top = __reduce_max_sync(0xffffffffu, top);
-            } else {
-#pragma unroll
-                for (uint32_t o = C::GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            }
-            if (kv && live && cached) {
-                const bool is_v = hj >= heads + kv_heads;
-                const uint64_t at = (block * kv_heads + (hj - heads - (is_v ? kv_heads : 0))) * Q8_BS + place;
-                float inv, s;
-                q8_scale(top, inv, s);
-                *reinterpret_cast<uint32_t*>((is_v ? v_pool : k_pool) + at * HD + 4 * l) = q8_pack4(x[j].x, x[j].y, x[j].z, x[j].w, inv, s == s);
-                if (l == 0) (is_v ? v_scales : k_scales)[at] = s;
-            }
         }
-        h += AP_AHEAD * C::GROUPS;
-        if (per_block > 1) break;
+        const bool kept = live && (uint32_t)slot < pool_slots;   // a key or value head with a place
+        if (!__any_sync(0xffffffffu, kept)) continue;
+        uint32_t top = 0;
+#pragma unroll
+        for (uint32_t c = 0; c < P; c++) top = max(top, max(max(abs_bits(x[c].x), abs_bits(x[c].y)), max(abs_bits(x[c].z), abs_bits(x[c].w))));
+#pragma unroll
+        for (uint32_t o = C::LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (kept) {
+            const bool is_v = head >= heads + kv_heads;
+            const uint64_t at = ((uint64_t)((uint32_t)slot / Q8_BS) * kv_heads + (head - heads - (is_v ? kv_heads : 0))) * Q8_BS + (uint32_t)slot % Q8_BS;
+            float inv, s;
+            q8_scale(top, inv, s);
+            int8_t* dst = (is_v ? v_pool : k_pool) + at * HD + 4 * l;
+#pragma unroll
+            for (uint32_t c = 0; c < P; c++) *reinterpret_cast<uint32_t*>(dst + c * STEP) = q8_pack4(x[c].x, x[c].y, x[c].z, x[c].w, inv, s == s);
+            if (l == 0) (is_v ? v_scales : k_scales)[at] = s;
+        }
     }
 }
 
@@ -507,10 +516,18 @@ kv_read_q8_kernel(const int8_t* __restrict__ k_pool, const int8_t* __restrict__ 
 template <typename T, int HD>
 static int append_q8(cudaStream_t st, const float* qkv, const float* rope, uint32_t rope_len, const int32_t* positions, const int32_t* slots, void* q_out,
                      int8_t* k_pool, int8_t* v_pool, float* k_scales, float* v_scales, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t pool_slots) {
-    const uint32_t total = heads + 2 * kv_heads, per_block = total >= ApCfg<HD>::GROUPS ? 1 : ApCfg<HD>::GROUPS / total;
+    const uint32_t total = heads + 2 * kv_heads;
+    // Tokens of a block: those of up to 4 turns that leave the fewest groups idle in the last one, while there are three blocks an SM (2000
+    // tokens of 20 heads of 128: 6.6 us with one a block, 6.4 with three).
+    uint32_t per_block = 1;
+    float best = 0.0f;
+    for (uint32_t n = 1; n == 1 || (n * total <= 4 * ApCfg<HD>::GROUPS && cdiv(tokens, n) >= 3 * B200_SMS); n++) {
+        const float used = (float)(n * total) / (float)(cdiv(n * total, ApCfg<HD>::GROUPS) * ApCfg<HD>::GROUPS);
+        if (used > 1.01f * best) { best = used; per_block = n; }
+    }
     return launch_k(rope_kv_append_q8_kernel<T, HD>, dim3(cdiv(tokens, per_block)), dim3(AP_THREADS), 0, st, NO_CLUSTER, qkv,
                     reinterpret_cast<const float4*>(rope), rope_len, positions, slots, (T*)q_out, k_pool, v_pool, k_scales, v_scales, tokens, heads, kv_heads,
-                    pool_slots, per_block);
+                    pool_slots, per_block, Q8Div(total));
 }
 
 template <typename T, int HD>
