@@ -523,23 +523,11 @@ static I8Plan i8_plan(uint32_t m, uint32_t n, uint32_t k) {
     return p;
 }
 
-template <typename K>
-static int i8_allow_smem(K* kernel, bool* set, uint32_t bytes) {
-    int dev = 0;
-    AK_CUDA(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lock(device_cache_mutex());
-    if (!set[dev & 63]) {
-        AK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        set[dev & 63] = true;
-    }
-    return AK_OK;
-}
-
 template <int EPI, bool SPLIT>
 static int i8_launch_tile(cudaStream_t st, const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmEpi& ep, const I8Scales& sc, uint32_t m, uint32_t n, uint32_t k,
                           const I8Plan& p) {
     static bool set[64] = {};
-    AK_TRY(i8_allow_smem(gemm_q8_kernel<EPI, SPLIT>, set, I8_SMEM_ONE));
+    AK_TRY(q8_allow_smem(gemm_q8_kernel<EPI, SPLIT>, set, I8_SMEM_ONE));
     const uint32_t ar = i8_slot_rows(m);
     uint32_t cols = 32;
     while (cols < p.bn) cols *= 2;
@@ -553,7 +541,7 @@ static int i8_launch_epi(cudaStream_t st, const void* a, const void* wt, const G
     const I8Plan p = i8_plan(m, n, k);
     if (!p.bn) {
         static bool set[64] = {};
-        AK_TRY(i8_allow_smem(gemm_q8_pair_kernel<EPI>, set, I8_SMEM_PAIR));
+        AK_TRY(q8_allow_smem(gemm_q8_pair_kernel<EPI>, set, I8_SMEM_PAIR));
         constexpr uint32_t OUT = I8P_EPI_WARPS * I8P_OUT_WARP, STAGES = (I8_SMEM_PAIR - 1024 - OUT) / I8P_STAGE;
         static_assert(STAGES >= 2 && STAGES <= I8_MAX_STAGES, "ring of the pair kernel");
         AK_TRY(make_tmap_2d(&tmA, a, 2, k / 2, m, k, I8_KB / 2, I8_M, TMA_SWIZZLE_128B));

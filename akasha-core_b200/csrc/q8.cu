@@ -18,11 +18,13 @@ int q8_check_here(const void* p, const char* who) {
 
 // ============================================================================ norm + quantisation
 // h = x (+ residual, written back), y = h / sqrt(mean(h^2) + eps) * w (w == nullptr: y = h), q = rint(127 y / max|y|), s = max|y| / 127.
-// One pass: a row lives in the registers of its threads between the two reductions (sum of squares, largest magnitude), so that every
-// input byte is read once and every output byte written once. `tpr` threads share a row.
+// The root divides every value of a row alike: q = rint(127 h w / max|h w|) does without it, and the sum of squares and the largest |h w| are taken
+// together, in one pass and with one exchange between the row's threads. A row lives in their registers from then on: every input byte is read
+// once, every output byte written once. `tpr` threads share a row.
 //
-// What bounds it once the bytes do not: instructions, some 200 of them per warp and row for the reductions and scales (IEEE divisions and roots
-// made that 300), so long rows take several values a thread and rows of up to 1024 values one warp.
+// What bounds it: the bytes (with a residual 1.0 of the copy bandwidth, 16384 x 2048 f32 26.8 us = 0.96, 4001 x 8192 26.0 = 0.96, in the
+// ring), and instructions where these are few (4001 x 8192 bf16 with weights 20.8 us = 0.72, rows of 2047 39.6 us = 0.65). With y itself and two
+// reductions, one after the other: 31, 38, 26.6 and 50 us.
 template <typename T> struct Q8Vec {
     static constexpr int V = 16 / sizeof(T);   // values of a group: a 16-byte load
     static __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
@@ -38,34 +40,55 @@ template <typename T> struct Q8Vec {
 
 constexpr uint32_t NQ_MAX_WARPS = 32;
 
-// The sum of a row's threads' values, in the same order in every thread; the largest of their (unsigned) values.
-__device__ __forceinline__ float row_sum(float v, float* s_sum, uint32_t warps, uint32_t wid, uint32_t lane) {
-    v = warp_sum(v);
-    if (warps == 1) return v;
-    if (lane == 0) s_sum[wid] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (uint32_t i = 0; i < warps; i++) v += s_sum[i];
-    return v;
+// The largest of |a|, |b| and |c|, NaN if one is NaN.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
-__device__ __forceinline__ uint32_t row_top(uint32_t v, uint32_t* s_top, uint32_t warps, uint32_t wid, uint32_t lane) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    if (warps == 1) return v;
-    if (lane == 0) s_top[wid] = v;
-    __syncthreads();
-    return __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
+// The sum (`norm`: if it is wanted) and the largest of the non-negative values of a row's threads, the same in every one. `both`: the row's warps' values.
+struct RowWarps {
+    float sum[NQ_MAX_WARPS];
+    uint32_t top[NQ_MAX_WARPS];
+};
+__device__ __forceinline__ void row_reduce(bool norm, float& sum, float& top, RowWarps& both, uint32_t warps, uint32_t wid, uint32_t lane) {
+    if (norm) sum = warp_sum(sum);
+    uint32_t bits = __reduce_max_sync(0xffffffffu, abs_bits(top));
+    if (warps > 1) {
+        if (lane == 0) { both.sum[wid] = sum; both.top[wid] = bits; }
+        __syncthreads();
+        if (norm) sum = warp_sum(lane < warps ? both.sum[lane] : 0.0f);
+        bits = __reduce_max_sync(0xffffffffu, lane < warps ? both.top[lane] : 0u);
+    }
+    top = __uint_as_float(bits);
+}
+// What a row's values h w (without weights: h) are multiplied by, and the row's scale, from the largest magnitude `top`: y = rs h w is larger by rs, which the
+// quotients do not see, so that the sum of squares and the largest value take one pass and one exchange.
+struct RowScale {
+    float inv, s;
+    bool ok;   // s is a number
+};
+__device__ __forceinline__ RowScale row_scale(bool norm, float sum, float top, float inv_size, float eps) {
+    const float y = norm ? top * rsqrtf(sum * inv_size + eps) : top;
+    const bool some = y >= Q8_ZERO && top >= 1e-36f;   // (127 / top would overflow)
+    float r;   // 128 / top, as in q8_scale
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top * 0.0078125f));
+    RowScale o;
+    o.ok = y < INFINITY;
+    o.inv = some && o.ok ? r * 0.9921875f : 0.0f;
+    o.s = !o.ok ? __uint_as_float(0x7fc00000u) : some ? y * (1.0f / 127.0f) : 0.0f;
+    return o;
 }
 
 // Rows of whole vectors: a thread holds NV groups of V consecutive values (16 bytes of input).
 template <typename T, int NV>
 __global__ void __launch_bounds__(1024)
 norm_q8_kernel(T* __restrict__ x, const float* __restrict__ residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales,
-               uint32_t rows, uint32_t size, float eps) {
+               uint32_t rows, uint32_t size, float inv_size, float eps) {
     constexpr int V = Q8Vec<T>::V;
     pdl_wait();
     pdl_trigger();
-    __shared__ float s_sum[NQ_MAX_WARPS];
-    __shared__ uint32_t s_top[NQ_MAX_WARPS];
+    __shared__ RowWarps both;
     const uint32_t tpr = blockDim.x, t = threadIdx.x, lane = t & 31, wid = t >> 5, warps = tpr >> 5, groups = size / V;
     const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;   // blockDim.y > 1 only with one warp per row
     if (row >= rows) return;
@@ -94,271 +117,271 @@ norm_q8_kernel(T* __restrict__ x, const float* __restrict__ residual, const floa
             }
         }
     }
+    float sum = 0.0f;
     if (w) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NV; c++)
-#pragma unroll
-            for (int e = 0; e < V; e++) ss += y[c][e] * y[c][e];
-        const float rs = rsqrtf(row_sum(ss, s_sum, warps, wid, lane) / (float)size + eps);
 #pragma unroll
         for (int c = 0; c < NV; c++) {
             const uint32_t g = t + c * tpr;
+#pragma unroll
+            for (int e = 0; e < V; e++) sum += y[c][e] * y[c][e];
             if (g >= groups) continue;
 #pragma unroll
             for (int k = 0; k < V; k += 4) {
                 float ww[4];
                 Q8Vec<float>::load(w + V * g + k, ww);
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[c][k + e] = y[c][k + e] * rs * ww[e];
+                for (int e = 0; e < 4; e++) y[c][k + e] *= ww[e];
             }
         }
     }
-    uint32_t top = 0;
+    float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < NV; c++)
 #pragma unroll
-        for (int e = 0; e < V; e++) top = max(top, abs_bits(y[c][e]));
-    float inv, s;
-    q8_scale(row_top(top, s_top, warps, wid, lane), inv, s);
-    const bool ok = s == s;
-    if (t == 0) scales[row] = s;
+        for (int e = 0; e < V; e += 2) top = max_abs(top, y[c][e], y[c][e + 1]);
+    row_reduce(w, sum, top, both, warps, wid, lane);
+    const RowScale sc = row_scale(w, sum, top, inv_size, eps);
+    if (t == 0) scales[row] = sc.s;
 #pragma unroll
     for (int c = 0; c < NV; c++) {
         const uint32_t g = t + c * tpr;
         if (g >= groups) continue;
         uint32_t o[V / 4];
 #pragma unroll
-        for (int k = 0; k < V / 4; k++) o[k] = q8_pack4(y[c][4 * k], y[c][4 * k + 1], y[c][4 * k + 2], y[c][4 * k + 3], inv, ok);
+        for (int k = 0; k < V / 4; k++) o[k] = q8_pack4(y[c][4 * k], y[c][4 * k + 1], y[c][4 * k + 2], y[c][4 * k + 3], sc.inv, sc.ok);
         if constexpr (V == 8) *reinterpret_cast<uint2*>(q + V * g) = make_uint2(o[0], o[1]);
         else *reinterpret_cast<uint32_t*>(q + V * g) = o[0];
     }
 }
 
-// Rows of any size. All the arrays of a row start at the same element offset, so groups are cut where the ADDRESS is a multiple of V elements; the
-// first and last group of a row are partial. With weights (KEEP), resident blocks walk over the rows with a stride that is a multiple of V, so that a block
-// sees one shift only: which of a thread's groups are partial and its weights (in registers) are settled once: 16384 x 2047 50 us, where a
-// block per row, its weights put together from two neighbouring vectors, took 56. Without weights there is nothing to keep, and with a
-// residual the loads want blocks coming and going.
-template <typename T, int NV, bool KEEP>
-__global__ void __launch_bounds__(KEEP ? 512 : 1024, KEEP ? 2 : 1)
-norm_q8_ragged_kernel(T* __restrict__ x, const float* __restrict__ residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales,
-                      uint32_t rows, uint32_t size, float eps) {
-    constexpr int V = Q8Vec<T>::V;
+constexpr uint32_t NQ_RING_BYTES = 226 * 1024;
+// Many rows: resident blocks walk over them, a block's next row on its way into shared memory while one is worked on, the weights in registers. A thread
+// copies what it reads itself: nobody waits for anybody's copy.
+// ODD: rows of any size. All the arrays of a row start at the same element offset, so groups are cut where the ADDRESS is a multiple of V elements, and
+// the first and the last group of a row may be partial. The blocks' stride is a multiple of V rows, so that a block sees one shift only, and which
+// of a thread's groups are partial is settled once.
+template <typename T, int NV, bool ODD, bool RES>
+__global__ void __launch_bounds__(1024)
+norm_q8_ring_kernel(T* __restrict__ x, const float* __restrict__ residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales,
+                    uint32_t rows, uint32_t size, float inv_size, float eps) {
+    constexpr int V = Q8Vec<T>::V, KINDS = RES ? 2 : 1;
     pdl_wait();
     pdl_trigger();
-    __shared__ float s_sum[NQ_MAX_WARPS];
-    __shared__ uint32_t s_top[2][NQ_MAX_WARPS];
+    extern __shared__ __align__(16) uint8_t ring[];       // [2][x, residual][group of a thread][thread] of 16 bytes
+    __shared__ RowWarps both[2];
     const uint32_t tpr = blockDim.x, t = threadIdx.x, lane = t & 31, wid = t >> 5, warps = tpr >> 5;
-    uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;   // blockDim.y > 1 only with one warp per row
-    if (row >= rows) return;
-    const uint32_t step = gridDim.x * blockDim.y;           // a multiple of V, or there is no second row
-    const uint32_t shift = (uint32_t)(((size_t)row * size) & (V - 1)), groups = (shift + size + V - 1) / V;
-    auto inside = [&](int32_t i) { return i >= 0 && (uint32_t)i < size; };
-    float ww[KEEP ? NV : 1][V];
-    bool some[NV], part[NV];
+    const uint32_t step = gridDim.x;                        // ODD: a multiple of V, or there is no second row
+    const uint32_t shift = ODD ? (uint32_t)(((size_t)blockIdx.x * size) & (V - 1)) : 0, groups = (shift + size + V - 1) / V;
+    auto inside = [&](uint32_t i) { return i - shift < size; };   // i: from the row's group 0 on
+    auto there = [&](int c) { return t + c * tpr < groups; };
+    float ww[NV][V];
+    uint32_t part = 0;   // bit c: group c is partial
 #pragma unroll
     for (int c = 0; c < NV; c++) {
-        const int32_t e0 = (int32_t)(V * (t + c * tpr) - shift);
-        some[c] = t + c * tpr < groups;
-        part[c] = some[c] && !(e0 >= 0 && (uint32_t)e0 + V <= size);
-        if constexpr (KEEP) {
+        const uint32_t i = V * (t + c * tpr);
 #pragma unroll
-            for (int e = 0; e < V; e++) ww[c][e] = inside(e0 + e) ? w[e0 + e] : 0.0f;
+        for (int e = 0; e < V; e++) ww[c][e] = 0.0f;
+        if (ODD && there(c) && !(inside(i) && inside(i + V - 1))) part |= 1u << c;
+        if (!w || !there(c)) continue;
+        if constexpr (ODD) {
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                if (inside(i + e)) ww[c][e] = w[i + e - shift];
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; k += 4) Q8Vec<float>::load(w + i + k, *reinterpret_cast<float(*)[4]>(&ww[c][k]));
         }
     }
-    for (uint32_t turn = 0; row < rows; row += step, turn ^= 1) {
-        const size_t off = (size_t)row * size - shift;   // of group 0 (which may begin in the row before)
-        T* xr = x + off;
-        int8_t* qr = q + off;
+    const uint32_t my = smem_u32(ring) + t * 16;
+    const size_t stride = (size_t)step * size, off0 = (size_t)blockIdx.x * size - shift + V * t;
+    // (a partial group is read whole, with neighbouring rows' values that are dropped, but not past the last row)
+    auto ask = [&](uint32_t row, size_t off, uint32_t half) {
+        if (row < rows) {
+#pragma unroll
+            for (int c = 0; c < NV; c++) {
+                if (!there(c)) continue;
+                uint32_t bytes = 16;
+                if (ODD && part && row + 1 == rows) bytes = min(16u, (shift + size - V * (t + c * tpr)) * (uint32_t)sizeof(T));
+#pragma unroll
+                for (int k = 0; k < KINDS; k++) {
+                    const void* src = k ? (const void*)(residual + off + c * V * tpr) : (const void*)(x + off + c * V * tpr);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(my + ((half * KINDS + k) * NV + c) * tpr * 16), "l"(src), "r"(bytes) : "memory");
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    ask(blockIdx.x, off0, 0);
+    size_t off = off0;
+    uint32_t half = 0;
+    for (uint32_t row = blockIdx.x; row < rows; row += step, off += stride, half ^= 1) {
+        ask(row + step, off + stride, half ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
         float y[NV][V];
 #pragma unroll
         for (int c = 0; c < NV; c++) {
-            const uint32_t at = V * (t + c * tpr);
+            const uint8_t* src = ring + t * 16 + ((half * KINDS) * NV + c) * tpr * 16;
 #pragma unroll
             for (int e = 0; e < V; e++) y[c][e] = 0.0f;
-            if (!some[c]) continue;
-            // a partial group is read whole too, with values of the neighbouring rows that are dropped, but for one that would reach past the last row
-            if (!part[c] || row + 1 < rows || at + V <= shift + size) Q8Vec<T>::load(xr + at, y[c]);
-            else {
+            if (!there(c)) continue;
+            Q8Vec<T>::load(reinterpret_cast<const T*>(src), y[c]);
+            if constexpr (RES) {
+                float r[4];
+                Q8Vec<float>::load(reinterpret_cast<const float*>(src + NV * tpr * 16), r);
 #pragma unroll
-                for (int e = 0; e < V; e++)
-                    if (at + e >= shift && at + e < shift + size) y[c][e] = Cvt<T>::to_f(xr[at + e]);
+                for (int e = 0; e < 4; e++) y[c][e] += r[e];
+                if (!ODD || !(part >> c & 1u)) *reinterpret_cast<float4*>(x + off + c * V * tpr) = make_float4(y[c][0], y[c][1], y[c][2], y[c][3]);
             }
         }
-        if constexpr (sizeof(T) == 4) {
-            if (residual) {
-                const float* rr = residual + off;
+        if (ODD && part) {
 #pragma unroll
-                for (int c = 0; c < NV; c++) {
-                    const uint32_t at = V * (t + c * tpr);
-                    if (!some[c]) continue;
-                    if (!part[c]) {
-                        float r[4];
-                        Q8Vec<float>::load(rr + at, r);
+            for (int c = 0; c < NV; c++)
+                if (part >> c & 1u) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) y[c][e] += r[e];
-                        *reinterpret_cast<float4*>(xr + at) = make_float4(y[c][0], y[c][1], y[c][2], y[c][3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < V; e++)
-                            if (at + e >= shift && at + e < shift + size) { y[c][e] += rr[at + e]; xr[at + e] = y[c][e]; }
+                    for (int e = 0; e < V; e++) {
+                        if (!inside(V * (t + c * tpr) + e)) y[c][e] = 0.0f;
+                        else if constexpr (RES) x[off + c * V * tpr + e] = y[c][e];
                     }
                 }
-            }
         }
-#pragma unroll
-        for (int c = 0; c < NV; c++)
-            if (part[c]) {
-#pragma unroll
-                for (int e = 0; e < V; e++)
-                    if (!inside((int32_t)(V * (t + c * tpr) - shift) + e)) y[c][e] = 0.0f;
-            }
+        float sum = 0.0f, top = 0.0f;
         if (w) {
-            float ss = 0.0f;
 #pragma unroll
             for (int c = 0; c < NV; c++)
 #pragma unroll
-                for (int e = 0; e < V; e++) ss += y[c][e] * y[c][e];
-            const float rs = rsqrtf(row_sum(ss, s_sum, warps, wid, lane) / (float)size + eps);
-#pragma unroll
-            for (int c = 0; c < NV; c++) {
-                const int32_t e0 = (int32_t)(V * (t + c * tpr) - shift);
-#pragma unroll
                 for (int e = 0; e < V; e++) {
-                    if constexpr (KEEP) y[c][e] = y[c][e] * rs * ww[c][e];
-                    else if (inside(e0 + e)) y[c][e] = y[c][e] * rs * w[e0 + e];
+                    sum += y[c][e] * y[c][e];
+                    y[c][e] *= ww[c][e];
                 }
-            }
         }
-        uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < NV; c++)
 #pragma unroll
-            for (int e = 0; e < V; e++) top = max(top, abs_bits(y[c][e]));
-        float inv, s;
-        q8_scale(row_top(top, s_top[turn], warps, wid, lane), inv, s);   // two buffers: a warp may be a row ahead of another that still reads
-        const bool ok = s == s;
-        if (t == 0) scales[row] = s;
+            for (int e = 0; e < V; e += 2) top = max_abs(top, y[c][e], y[c][e + 1]);
+        row_reduce(w, sum, top, both[half], warps, wid, lane);   // two: a warp may be a row ahead of another that still reads
+        const RowScale sc = row_scale(w, sum, top, inv_size, eps);
+        if (t == 0) scales[row] = sc.s;
+        uint32_t o[NV][V / 4];
 #pragma unroll
         for (int c = 0; c < NV; c++) {
-            const uint32_t at = V * (t + c * tpr);
-            if (!some[c]) continue;
-            uint32_t o[V / 4];
 #pragma unroll
-            for (int k = 0; k < V / 4; k++) o[k] = q8_pack4(y[c][4 * k], y[c][4 * k + 1], y[c][4 * k + 2], y[c][4 * k + 3], inv, ok);
-            if (!part[c]) {
-                if constexpr (V == 8) *reinterpret_cast<uint2*>(qr + at) = make_uint2(o[0], o[1]);
-                else *reinterpret_cast<uint32_t*>(qr + at) = o[0];
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; e++)
-                    if (at + e >= shift && at + e < shift + size) qr[at + e] = (int8_t)(o[e / 4] >> (8 * (e % 4)));
-            }
+            for (int k = 0; k < V / 4; k++) o[c][k] = q8_pack4(y[c][4 * k], y[c][4 * k + 1], y[c][4 * k + 2], y[c][4 * k + 3], sc.inv, sc.ok);
+            if (!there(c) || (ODD && (part >> c & 1u))) continue;
+            int8_t* dst = q + off + c * V * tpr;
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(o[c][0], o[c][1]);
+            else *reinterpret_cast<uint32_t*>(dst) = o[c][0];
         }
-        if (!KEEP) break;
+        if (ODD && part) {
+#pragma unroll
+            for (int c = 0; c < NV; c++)
+                if (part >> c & 1u) {
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        if (inside(V * (t + c * tpr) + e)) q[off + c * V * tpr + e] = (int8_t)(o[c][e / 4] >> (8 * (e % 4)));
+                }
+        }
     }
 }
 
-// Rows that do not fit the registers of a block, and buffers that are not aligned for vectors: a block per row, three passes over it (the second and
-// third read what the first wrote back). y is computed twice by the same operations, hence with the same bits.
+// Rows that do not fit the registers of a block, and buffers that are not aligned for vectors: a block per row, two passes over it (the second reads what
+// the first wrote back).
 template <typename T>
 __global__ void __launch_bounds__(1024)
-norm_q8_any_kernel(T* x, const float* residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales, uint32_t size, float eps) {
+norm_q8_any_kernel(T* x, const float* residual, const float* __restrict__ w, int8_t* __restrict__ q, float* __restrict__ scales, uint32_t size, float inv_size, float eps) {
     pdl_wait();
     pdl_trigger();
-    __shared__ float s_sum[NQ_MAX_WARPS];
-    __shared__ uint32_t s_top[NQ_MAX_WARPS];
+    __shared__ RowWarps both;
     const uint32_t lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const size_t off = (size_t)blockIdx.x * size;
-    float ss = 0.0f;
+    float sum = 0.0f;
+    float top = 0.0f;
     for (uint32_t i = threadIdx.x; i < size; i += blockDim.x) {
         float v = Cvt<T>::to_f(x[off + i]);
         if constexpr (sizeof(T) == 4) {
             if (residual) { v += residual[off + i]; x[off + i] = v; }
         }
-        ss += v * v;
+        sum += v * v;
+        top = max_abs(top, w ? v * w[i] : v, 0.0f);
     }
-    float rs = 1.0f;
-    if (w) {
-        ss = warp_sum(ss);
-        if (lane == 0) s_sum[wid] = ss;
-        __syncthreads();
-        ss = warp_sum(lane < warps ? s_sum[lane] : 0.0f);
-        rs = rsqrtf(ss / (float)size + eps);
+    row_reduce(w, sum, top, both, warps, wid, lane);
+    const RowScale sc = row_scale(w, sum, top, inv_size, eps);
+    if (threadIdx.x == 0) scales[blockIdx.x] = sc.s;
+    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x) {
+        const float v = Cvt<T>::to_f(x[off + i]);   // (what this thread wrote back)
+        q[off + i] = q8_of(w ? v * w[i] : v, sc.inv, sc.ok);
     }
-    auto value = [&](uint32_t i) { return w ? Cvt<T>::to_f(x[off + i]) * rs * w[i] : Cvt<T>::to_f(x[off + i]); };   // written by this thread
-    uint32_t top = 0;
-    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x) top = max(top, abs_bits(value(i)));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) s_top[wid] = top;
-    __syncthreads();
-    top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
-    float inv, s;
-    q8_scale(top, inv, s);
-    const bool ok = s == s;
-    if (threadIdx.x == 0) scales[blockIdx.x] = s;
-    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x) q[off + i] = q8_of(value(i), inv, ok);
 }
 
 template <typename T>
 static int norm_q8(cudaStream_t st, T* x, const float* residual, const float* w, int8_t* q, float* scales, uint32_t rows, uint32_t size, float eps) {
     constexpr uint32_t V = Q8Vec<T>::V, MOST = 32 / V;   // 32 values a thread
     const uint32_t groups = cdiv(size, V) + (size % V ? 1 : 0);   // of a row, at most
+    const float inv_size = 1.0f / (float)size;
     const bool vectors = q8_aligned(x, 16) && q8_aligned(residual, 16) && q8_aligned(q, V) && q8_aligned(w, 16);
-    if (!vectors || groups > 1024 * (size % V ? MOST / 2 : MOST))
-        return launch_k(norm_q8_any_kernel<T>, dim3(rows), dim3(512), 0, st, NO_CLUSTER, x, residual, w, q, scales, size, eps);
+    if (!vectors)
+        return launch_k(norm_q8_any_kernel<T>, dim3(rows), dim3(512), 0, st, NO_CLUSTER, x, residual, w, q, scales, size, inv_size, eps);
     const bool few = rows <= 2 * B200_SMS;   // latency: as many threads to a row as there are vectors
-    if (size % V) {
-        uint32_t n = few ? 1 : groups <= 32 * MOST / 2 ? cdiv(groups, 32) : MOST / 2;   // 16 values a thread
-        if (n == 3) n = 4;
-        while (groups > n * 1024) n *= 2;
-        const uint32_t tpr = cdiv(groups, n * 32) * 32;
-        const dim3 block(tpr, tpr == 32 && !few ? 4 : 1);
-        const bool keep = w && !residual && !few && tpr <= 512;
-#define AK_NORM_Q8(N)                                                                                                                                         \
-    case N: {                                                                                                                                                 \
-        const uint32_t blocks = cdiv(rows, block.y);                                                                                                          \
-        if (!keep) return launch_k(norm_q8_ragged_kernel<T, N, false>, dim3(blocks), block, 0, st, NO_CLUSTER, x, residual, w, q, scales, rows, size, eps);   \
-        int occ = 0;                                                                                                                                          \
-        AK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, norm_q8_ragged_kernel<T, N, true>, (int)(block.x * block.y), 0));                         \
-        const uint32_t most = B200_SMS * (uint32_t)(occ < 1 ? 1 : occ) / V * V;                                                                               \
-        return launch_k(norm_q8_ragged_kernel<T, N, true>, dim3(blocks < most ? blocks : most), block, 0, st, NO_CLUSTER, x, residual, w, q, scales, rows,    \
-                        size, eps);                                                                                                                           \
-    }
-        switch (n) {
-            AK_NORM_Q8(1);
-            AK_NORM_Q8(2);
-        }
-        if constexpr (MOST == 8) {
-            switch (n) { AK_NORM_Q8(4); }
-        }
+    const bool odd = size % V != 0;
+    // The ring: any odd size; with weights, rows of more than 24 values a lane of one warp (16384 x 1024 f32 14.9 us, in the other kernel 17.4, but 768 12.5
+    // and 12.3), enough of them to keep the resident blocks busy (1000 x 4096 f32 4.3 and 4.1). A residual or no weights leave nothing
+    // to keep, and then blocks that come and go are as good or better (16384 x 2048 f32 with a residual 65 us, 72 in the ring).
+    if (odd || (w && !residual && rows >= 16 * B200_SMS && size > 768)) {
+        // 16 values a thread, few rows or short ones fewer
+        const uint32_t n = groups <= (few ? 1024 : 32) ? 1 : groups <= (few ? 2048 : 64) ? 2 : 16 / V, tpr = cdiv(groups, n * 32) * 32;
+        const uint32_t bytes = 2 * n * tpr * 16 * (residual ? 2 : 1);   // of shared memory
+        if (tpr <= 1024 && bytes <= NQ_RING_BYTES) {
+#define AK_NORM_Q8(N, ODD, RES)                                                                                                                                \
+    do {                                                                                                                                                       \
+        static bool set[64] = {};                                                                                                                              \
+        AK_TRY(q8_allow_smem(norm_q8_ring_kernel<T, N, ODD, RES>, set, NQ_RING_BYTES));                                                                        \
+        uint32_t most = B200_SMS / V * V;                                                                                                                      \
+        if (rows > most) {   /* resident blocks */                                                                                                             \
+            int occ = 0;                                                                                                                                       \
+            AK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, norm_q8_ring_kernel<T, N, ODD, RES>, (int)tpr, bytes));                                \
+            most = B200_SMS * (uint32_t)(occ < 1 ? 1 : occ) / V * V;                                                                                           \
+        }                                                                                                                                                      \
+        return launch_k(norm_q8_ring_kernel<T, N, ODD, RES>, dim3(rows < most ? rows : most), dim3(tpr), bytes, st, NO_CLUSTER, x, residual, w, q, scales,     \
+                        rows, size, inv_size, eps);                                                                                                            \
+    } while (0)
+#define AK_NORM_Q8_ODD(N)                                       \
+    do {                                                        \
+        if constexpr (V == 4) {                                 \
+            if (residual) AK_NORM_Q8(N, true, true);            \
+        }                                                       \
+        AK_NORM_Q8(N, true, false);                             \
+    } while (0)
+            if (!odd) AK_NORM_Q8(16 / V, false, false);
+            if (n == 1) AK_NORM_Q8_ODD(1);
+            if (n == 2) AK_NORM_Q8_ODD(2);
+            if constexpr (V == 4) AK_NORM_Q8_ODD(4);
+#undef AK_NORM_Q8_ODD
 #undef AK_NORM_Q8
-    } else {
-        // Many rows: a warp each up to 32 values a thread (16384 x 768 f32 13 us, with 64 threads a row 19), but not with a residual, whose
-        // loads want more threads (26 against 32 us); long ones 16 values a thread, or 8 with a residual (16384 x 2048 31 us against
-        // 39 with 8; with a residual 65.2 us against 67.0 with 16).
-        uint32_t n = few ? 1 : residual ? 2 : groups <= 32 * MOST ? cdiv(groups, 32) : 16 / V;
-        if (n == 5 || n == 7) n++;
-        while (groups > n * 1024) n *= 2;
-        const uint32_t tpr = cdiv(groups, n * 32) * 32;
-        const dim3 block(tpr, tpr == 32 && !few ? 4 : 1);
+        }
+    }
+    if (odd || groups > 1024 * MOST)
+        return launch_k(norm_q8_any_kernel<T>, dim3(rows), dim3(512), 0, st, NO_CLUSTER, x, residual, w, q, scales, size, inv_size, eps);
+    // Many rows: a warp each up to 32 values a thread (16384 x 768 f32 12 us, with 64 threads a row 19), but not with a residual, whose loads want more
+    // threads (26 against 32 us); long ones 16 values a thread, or 8 with a residual (16384 x 2048: 65.0 us, with 16 65.8).
+    uint32_t n = few ? 1 : residual ? 2 : groups <= 32 * MOST ? cdiv(groups, 32) : 16 / V;
+    if (n == 5 || n == 7) n++;
+    while (groups > n * 1024) n *= 2;
+    const uint32_t tpr = cdiv(groups, n * 32) * 32;
+    const dim3 block(tpr, tpr == 32 && !few ? 4 : 1);
 #define AK_NORM_Q8(N) \
-    case N: return launch_k(norm_q8_kernel<T, N>, dim3(cdiv(rows, block.y)), block, 0, st, NO_CLUSTER, x, residual, w, q, scales, rows, size, eps)
-        switch (n) {
-            AK_NORM_Q8(1);
-            AK_NORM_Q8(2);
-            AK_NORM_Q8(3);
-            AK_NORM_Q8(4);
-        }
-        if constexpr (MOST == 8) {
-            switch (n) {
-                AK_NORM_Q8(6);
-                AK_NORM_Q8(8);
-            }
-        }
-#undef AK_NORM_Q8
+    case N: return launch_k(norm_q8_kernel<T, N>, dim3(cdiv(rows, block.y)), block, 0, st, NO_CLUSTER, x, residual, w, q, scales, rows, size, inv_size, eps)
+    switch (n) {
+        AK_NORM_Q8(1);
+        AK_NORM_Q8(2);
+        AK_NORM_Q8(3);
+        AK_NORM_Q8(4);
     }
+    if constexpr (MOST == 8) {
+        switch (n) {
+            AK_NORM_Q8(6);
+            AK_NORM_Q8(8);
+        }
+    }
+#undef AK_NORM_Q8
     set_error("ak_rmsnorm_q8: no kernel for rows of %u", size);
     return AK_ERR_UNSUPPORTED;
 }

@@ -34,6 +34,19 @@ static inline bool q8_head_dim_ok(uint32_t hd) { return hd == 32 || hd == 64 || 
 
 #ifdef __CUDACC__
 
+// Dynamic shared memory of a kernel, asked for once on each device (`set`: the kernel's own).
+template <typename K>
+inline int q8_allow_smem(K* kernel, bool* set, uint32_t bytes) {
+    int dev = 0;
+    AK_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(device_cache_mutex());
+    if (!set[dev & 63]) {
+        AK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        set[dev & 63] = true;
+    }
+    return AK_OK;
+}
+
 // A row y is held as q = rint(127 y / max|y|) and s = max|y| / 127. `top` is max|y| as the bits of a non-negative float: ordered as
 // unsigned integers these put infinity above every finite value and NaN above infinity, so that neither is lost in a maximum.
 // Rows whose largest value is under Q8_ZERO (127 / max would overflow) are zeros, s = 0; a row with an infinity or a NaN has s = NaN

@@ -275,8 +275,9 @@ AK_API int ak_bf16_to_f32(void* stream, const void* src, float* dst, uint64_t n)
 /* ---- 8-bit operators (no counterpart in the reference) ----
  * A row of numbers y is held as int8 values q = rint(127 y / max|y|) in -127..127 and one f32 scale s = max|y| / 127: y ~ q s, off by at
  * most s / 2. Rows are a token's activations, an output channel's weights, or one head's key or value at one cached position. A row whose
- * largest magnitude is under 1e-30 is held as zeros with s = 0; one with an infinity or a NaN as zeros with s = NaN, so that whatever is
- * computed from it is NaN. A call whose output (or, for the cache, key pool) lies on another device than the current one, or in memory that no
+ * largest magnitude is under 1e-30 is held as zeros with s = 0 (under the norm also one whose largest h w, before the root divides it, is under
+ * 1e-36); one with an infinity or a NaN (under the norm: in h w) as zeros with s = NaN, so that whatever is computed from it is NaN. A call whose
+ * output (or, for the cache, key pool) lies on another device than the current one, or in memory that no
  * kernel can reach, returns AK_ERR_INVALID_ARG; all buffers of a call belong on the same device. Nothing is kept between calls, no
  * workspace is needed, and every call may be captured into a graph. Results do not depend on timing: the same call gives the same bits. */
 
@@ -284,7 +285,7 @@ AK_API int ak_bf16_to_f32(void* stream, const void* src, float* dst, uint64_t n)
  *   h = x + residual (residual != NULL: f32 x only; h is written back to x), y = h * rsqrt(mean(h^2) + eps) * w per row, q and scales as above.
  *   w == NULL: y = h, the rows are quantised as they are (weights [n,k] for ak_gemm_q8, activations behind SiLU or attention).
  * x [seq_len, size] f32 or bf16 (in_dtype); residual f32, w f32 [size]; q int8 [seq_len, size]; scales f32 [seq_len]. Any size;
- * rows of up to 32768 values (sizes that are no multiple of 16 bytes of x: 16376) are read once if x, residual and w are 16-byte aligned and q to the bytes of 16 bytes of x (4, bf16 8),
+ * rows of up to 32768 values (sizes that are no multiple of 16 bytes of x: 14000) are read once if x, residual and w are 16-byte aligned and q to the bytes of 16 bytes of x (4, bf16 8),
  * others run element by element. */
 AK_API int ak_rmsnorm_q8(void* stream, void* x, uint32_t in_dtype, const float* residual, const float* w, int8_t* q, float* scales, ak_norm_meta m);
 

@@ -41,7 +41,7 @@ def _check_rows(torch, y, tol, q, scales):
 
 
 @pytest.mark.parametrize("rows,size", [(1, 1), (1, 3), (3, 7), (2, 65), (64, 768), (5, 320), (130, 1001), (297, 64), (300, 2048), (301, 2047), (297, 129), (7, 8192),
-                                       (300, 8190), (2, 32765), (2, 32768), (3, 33001), (2, 40000)])
+                                       (300, 8190), (2, 32765), (2, 32768), (3, 33001), (2, 40000), (2400, 1024), (5003, 1001), (2500, 5001), (700, 14001), (5001, 37)])
 @pytest.mark.parametrize("form", ["residual", "plain", "rows", "bf16", "bf16_rows"])
 def test_norm(ak, torch_cuda, rows, size, form):
     torch = torch_cuda
@@ -106,6 +106,41 @@ def test_rows_without_a_scale(ak, torch_cuda, size, norm):
         none = [1, 3, 4]
         _check_rows(torch, x[2:3].double() / math.sqrt(1e-5), _norm_error(size), q[2:3], scales[2:3])
     assert (q[none] == 0).all() and (scales[none[:-2]] == 0).all() and scales[3:5].isnan().all()
+
+
+@pytest.mark.parametrize("rows,size", [(2500, 1001), (2400, 2048), (9, 1003), (300, 64)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_between_rows_without_a_scale(ak, torch_cuda, rows, size, dtype):
+    """Every third row holds NaN or infinities only: nothing of it reaches its neighbours, which share 16-byte words with it in odd sizes."""
+    torch = torch_cuda
+    dt, tdt = _dt(ak, torch, dtype)
+    x = torch.randn(rows, size, device="cuda", generator=_gen(torch, rows)).to(tdt)
+    x[1::3] = float("nan")
+    x[4::6] = math.inf
+    w = 1 + 0.2 * torch.randn(size, device="cuda", generator=_gen(torch, 3))
+    q, scales = torch.full((rows, size), 77, dtype=torch.int8, device="cuda"), torch.full((rows,), 7.0, device="cuda")
+    ak.ops.rmsnorm_q8(x, None, w, q, scales, rows, size, 1e-5, in_dtype=dt)
+    torch.cuda.synchronize()
+    assert (q[1::3] == 0).all() and scales[1::3].isnan().all()
+    keep = torch.arange(rows, device="cuda") % 3 != 1
+    y = x[keep].double()
+    _check_rows(torch, y / ((y * y).mean(1, keepdim=True) + 1e-5).sqrt() * w.double(), _norm_error(size), q[keep], scales[keep])
+
+
+@pytest.mark.parametrize("size", [64, 67])
+def test_norm_of_small_products(ak, torch_cuda, size):
+    """Without eps a row may be tiny and y ordinary. h w of 1e-35 is a row like any other, under 1e-36 it counts as zero."""
+    torch = torch_cuda
+    x = torch.randn(2, size, device="cuda", generator=_gen(torch, 1)).clamp(-3, 3)
+    x[0] *= 1e-15
+    x[1] *= 1e-18
+    w = torch.full((size,), 1e-20, device="cuda")
+    q, scales = torch.full((2, size), 77, dtype=torch.int8, device="cuda"), torch.full((2,), 7.0, device="cuda")
+    ak.ops.rmsnorm_q8(x, None, w, q, scales, 2, size, 0.0)
+    torch.cuda.synchronize()
+    y = x[:1].double()
+    _check_rows(torch, y / (y * y).mean(1, keepdim=True).sqrt() * w.double(), _norm_error(size), q[:1], scales[:1])
+    assert (q[1] == 0).all() and scales[1] == 0
 
 
 # ------------------------------------------------------------------ product
