@@ -32,6 +32,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kernels.h"
 #include "q8.cuh"
 #include "tcgen05.cuh"
@@ -621,44 +623,99 @@ attn_decode_q8_kernel(const AqArgs a) {
     cluster.sync();   // nobody leaves while a peer may still read its results
 }
 
-// Warps of a CTA and splits of a sequence, for `room` warps on all SMs together.
+// ============================================================================ launch
+constexpr uint32_t AQ_ALONE = 120 * 1024;   // bytes of shared memory with which a CTA has an SM to itself
+
+template <typename T, int HD, int NQ, bool TWO> struct AqForm {
+    static constexpr uint32_t ROWS = 4 * NQ;
+    using C = AqCfg<HD>;
+    static constexpr size_t MERGE = (size_t)ROWS * HD * 4, RING = (size_t)C::STAGES * C::STAGE, PER_WARP = MERGE > RING ? MERGE : RING;
+    static constexpr size_t MOST = PER_WARP * AQ_MAX_WARPS > AQ_ALONE ? PER_WARP * AQ_MAX_WARPS : AQ_ALONE;
+    static size_t smem(uint32_t warps, bool alone) { return alone && PER_WARP * warps < AQ_ALONE ? AQ_ALONE : PER_WARP * warps; }
+
+    // Clusters of n CTAs of 8 warps that the device holds at once (asked for once; `alone`: one CTA on an SM).
+    static int room(int dev, uint32_t n, bool alone, uint32_t& clusters) {
+        static std::atomic<int> known[64][2][AQ_MAX_SPLITS + 1] = {};   // one more than the number
+        int k = known[dev & 63][alone][n].load(std::memory_order_relaxed);
+        if (!k) {
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
+            attr.val.clusterDim.z = n;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(B200_SMS, 1, n);
+            cfg.blockDim = dim3(AQ_MAX_WARPS * 32);
+            cfg.dynamicSmemBytes = smem(AQ_MAX_WARPS, alone);
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int num = 0;
+            AK_CUDA(cudaOccupancyMaxActiveClusters(&num, attn_decode_q8_kernel<T, HD, NQ, TWO>, &cfg));
+            known[dev & 63][alone][n].store(k = num + 1, std::memory_order_relaxed);
+        }
+        clusters = (uint32_t)(k - 1);
+        return AK_OK;
+    }
+};
+
+// Warps of a CTA, splits of a sequence, and whether its CTAs get an SM each.
+//
 // 8 warps instead of 4 where the sequences are long (128 blocks and more: the CTAs' starts and ends weigh less; 64 x 16 heads x 128 up to
 // 4096 positions 90 against 95 us, but 64 x 12 heads x 64 up to 512 16.4 against 13.0) or where all of them fit at once (8 x 12 heads 6.0 against
 // 6.6 us).
-// Split while that leaves 16 tiles to a warp and every CTA finds room at once (8 kv heads x 2 tiles of queries x 2 sequences of 60000: 93 us in 4, 63 in
-// 8, 90 in 16). Halves may take two waves (32 x 8 heads up to 8192: 58 us whole, 53 halved, 59 in quarters: ragged sequences end at different
-// times, and an exchange costs about a microsecond, hidden only behind other CTAs' streams).
-static void aq_plan(uint64_t units, uint32_t max_blocks, uint32_t room, uint32_t& warps, uint32_t& n_splits) {
-    warps = max_blocks >= 128 || units * 8 <= room ? 8 : 4;
-    if (n_splits) return;
-    n_splits = 1;
-    while (n_splits < AQ_MAX_SPLITS && units * warps * (n_splits == 1 ? 1 : 2 * n_splits) <= room && max_blocks / (2 * n_splits * warps) >= 16) n_splits *= 2;
+//
+// Splits: the number with the shortest estimate, in us, for sequences that fill half of their tables, fitted to 1 to 24 sequences of 500 to
+// 60000 positions: a wave of k CTAs on an SM takes 5 (clusters 6 and 0.06 for every CTA), and for each of a warp's tiles 0.2 + 0.002 HD times k
+// (1.15 for one alone: latency), or what its bytes take at 6.5 MB/us (once for all tiles of queries). Clusters share SMs before all are taken: `alone`
+// keeps a second CTA off an SM where all clusters find room like that. Measured whole and in what it picks: 1 x 12 heads x 64 x 4000 18.3 and
+// 8.4 us (8), 2 x 5 x 32 x 9000 9.0 (9), 5 x 8 kv heads x 128 x 30000 120 and 53 (3; 60 in 4), 24 x 8 x 128 x 6000 52 whole, 63 in 2. Over the 90 shapes
+// it is 4 % from the best number on average, 19 % at most (4 x 12 x 64 x 8000).
+template <typename F, int HD>
+static int aq_plan(uint64_t units, uint32_t q_tiles, uint32_t max_blocks, uint32_t& warps, uint32_t& n_splits, bool& alone) {
+    const uint32_t cap = F::C::CTAS * B200_SMS;   // CTAs of 8 warps on all SMs
+    warps = max_blocks >= 128 || units <= cap ? 8 : 4;
+    alone = false;
+    if (n_splits == 1 || (n_splits == 0 && warps == 4)) { n_splits = 1; return AK_OK; }
+    const float tile = 0.2f + 0.002f * HD, bytes = 8.0f * F::C::STAGE / (6.5e6f * (float)q_tiles);
+    const uint32_t blocks = (max_blocks + 1) / 2;
+    int dev = 0;
+    AK_CUDA(cudaGetDevice(&dev));
+    float best = 1e30f;
+    uint32_t pick = 1;
+    for (uint32_t n = n_splits ? n_splits : 1; n <= (n_splits ? n_splits : AQ_MAX_SPLITS) && (n == 1 || n_splits || blocks >= n * 8); n++) {
+        uint32_t room = cap, lone = 0;
+        if (n > 1) {
+            AK_TRY(F::room(dev, n, true, lone));
+            AK_TRY(F::room(dev, n, false, room));
+            if (room == 0) continue;
+        }
+        const bool one = n > 1 && units <= lone;
+        const float tiles = (float)cdiv(blocks, n * warps), fixed = n == 1 ? 5.0f : 6.0f + 0.06f * n;
+        auto wave = [&](uint64_t u) {
+            const uint32_t deep = (uint32_t)((u * n + B200_SMS - 1) / B200_SMS), k = one ? 1 : n > 1 && deep < 2 ? 2 : deep;
+            const float work = tile * (k > 1 ? (float)k : 1.15f), flow = bytes * (float)(u * n);
+            return fixed + tiles * (work > flow ? work : flow);
+        };
+        const uint64_t full = units / room;
+        const float t = (float)full * wave(room) + (units % room ? wave(units % room) : 0.0f);
+        if (t < 0.97f * best) { best = t; pick = n; alone = one; }
+    }
+    n_splits = pick;
+    return AK_OK;
 }
 
 template <typename T, int HD, int NQ, bool TWO>
 static int aq_launch(cudaStream_t st, AqArgs a, uint32_t rows, uint32_t n_splits) {
-    constexpr uint32_t ROWS = 4 * NQ;
-    using C = AqCfg<HD>;
-    constexpr size_t merge = (size_t)ROWS * HD * 4, ring = (size_t)C::STAGES * C::STAGE, per_warp = merge > ring ? merge : ring;
-    a.q_tiles = cdiv(a.q_len * a.group, ROWS);
+    using F = AqForm<T, HD, NQ, TWO>;
+    a.q_tiles = cdiv(a.q_len * a.group, F::ROWS);
     const uint64_t units = (uint64_t)rows * a.kv_heads * a.q_tiles;
     AK_REQUIRE(units <= 0x7fffffffu, AK_ERR_UNSUPPORTED, "ak_attn_decode_paged_q8: %u rows x %u heads x %u tiles of queries are too many for one call", rows,
                a.kv_heads, a.q_tiles);
+    static bool set[64] = {};
+    AK_TRY(q8_allow_smem(attn_decode_q8_kernel<T, HD, NQ, TWO>, set, (uint32_t)F::MOST, true));
     uint32_t warps;
-    while (n_splits & (n_splits - 1)) n_splits &= n_splits - 1;   // a cluster of a power of two of CTAs
-    aq_plan(units, a.max_blocks, C::CTAS * AQ_MAX_WARPS * B200_SMS, warps, n_splits);
-    {
-        static bool attr_set[64] = {};
-        int dev = 0;
-        AK_CUDA(cudaGetDevice(&dev));
-        std::lock_guard<std::mutex> lock(device_cache_mutex());
-        if (!attr_set[dev & 63]) {
-            AK_CUDA(cudaFuncSetAttribute(attn_decode_q8_kernel<T, HD, NQ, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(per_warp * AQ_MAX_WARPS)));
-            AK_CUDA(cudaFuncSetAttribute(attn_decode_q8_kernel<T, HD, NQ, TWO>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            attr_set[dev & 63] = true;
-        }
-    }
-    return launch_k(attn_decode_q8_kernel<T, HD, NQ, TWO>, dim3((unsigned)units, 1, n_splits), dim3(warps * 32), per_warp * warps, st,
+    bool alone;
+    AK_TRY((aq_plan<F, HD>(units, a.q_tiles, a.max_blocks, warps, n_splits, alone)));
+    return launch_k(attn_decode_q8_kernel<T, HD, NQ, TWO>, dim3((unsigned)units, 1, n_splits), dim3(warps * 32), F::smem(warps, alone), st,
                     n_splits > 1 ? dim3(1, 1, n_splits) : NO_CLUSTER, a);
 }
 

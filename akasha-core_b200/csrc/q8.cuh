@@ -34,14 +34,15 @@ static inline bool q8_head_dim_ok(uint32_t hd) { return hd == 32 || hd == 64 || 
 
 #ifdef __CUDACC__
 
-// Dynamic shared memory of a kernel, asked for once on each device (`set`: the kernel's own).
+// Dynamic shared memory of a kernel, and clusters of 16 CTAs, asked for once on each device (`set`: the kernel's own).
 template <typename K>
-inline int q8_allow_smem(K* kernel, bool* set, uint32_t bytes) {
+inline int q8_allow_smem(K* kernel, bool* set, uint32_t bytes, bool wide_clusters = false) {
     int dev = 0;
     AK_CUDA(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(device_cache_mutex());
     if (!set[dev & 63]) {
         AK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        if (wide_clusters) AK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         set[dev & 63] = true;
     }
     return AK_OK;

@@ -422,7 +422,7 @@ def test_attn_of_several_new_tokens(ak, torch_cuda, dtype, q_len, heads, kv_head
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("n_splits", [1, 2, 3, 4, 8, 16])
+@pytest.mark.parametrize("n_splits", [1, 2, 3, 4, 5, 7, 8, 11, 13, 16])
 def test_attn_splits(ak, torch_cuda, dtype, n_splits):
     """Any number of splits, most of them empty for the short sequences."""
     _attn(ak, torch_cuda, [0, 1, 40, 700, 3001], 2, 6, 3, 64, dtype, n_splits)
@@ -433,6 +433,8 @@ def test_attn_splits(ak, torch_cuda, dtype, n_splits):
 def test_attn_long(ak, torch_cuda, dtype):
     _attn(ak, torch_cuda, [40000], 1, 2, 2, 64, dtype)
     _attn(ak, torch_cuda, [30011, 9], 4, 8, 2, 128, dtype)
+    _attn(ak, torch_cuda, [4000, 2001, 17], 1, 12, 12, 64, dtype)
+    _attn(ak, torch_cuda, [6000] * 5, 1, 10, 5, 96, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
