@@ -24,7 +24,7 @@
 // Measured (graph of launches on three sets of inputs, cold L2): 64 sequences x 16 heads x 128, 64 to 4096 positions 90 us = 0.96 of the copy
 // bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 22.6 us = 0.73: bound by instructions there (some 210 a tile of 2176 bytes, issue
 // slots three quarters busy); 2 sequences of 60000 x 8 kv heads x 16 query rows 63 us = 0.59: few CTAs, instructions; one sequence of 300 x 5 heads
-// 5.8 us, a chain of latencies (an empty launch takes 2).
+// 5.8 us, a chain of latencies (the shortest launch takes 1.3).
 //
 // A CTA takes one (sequence, kv head, tile of queries, split); each warp has every n-th cache block of the split and a ring of cp.async
 // stages of its own, no barrier in the loop. The warps' results are merged in shared memory and the splits', which are the CTAs of one
