@@ -108,6 +108,21 @@ def test_rows_without_a_scale(ak, torch_cuda, size, norm):
     assert (q[none] == 0).all() and (scales[none[:-2]] == 0).all() and scales[3:5].isnan().all()
 
 
+@pytest.mark.parametrize("size", [4000, 4001])
+def test_norm_of_more_than_32_bits_of_values(ak, torch_cuda, size):
+    torch = torch_cuda
+    rows, n = 1100000, 5
+    x = torch.zeros(rows, size, dtype=torch.bfloat16, device="cuda")
+    x[-n:] = torch.randn(n, size, device="cuda", generator=_gen(torch, 1)).bfloat16()
+    w = 1 + 0.2 * torch.randn(size, device="cuda", generator=_gen(torch, 2))
+    q, scales = torch.full((rows, size), 77, dtype=torch.int8, device="cuda"), torch.full((rows,), 7.0, device="cuda")
+    ak.ops.rmsnorm_q8(x, None, w, q, scales, rows, size, in_dtype=ak.AK_BF16)
+    torch.cuda.synchronize()
+    y = x[-n:].double()
+    _check_rows(torch, y / ((y * y).mean(1, keepdim=True) + 1e-5).sqrt() * w.double(), _norm_error(size), q[-n:], scales[-n:])
+    assert (scales[:-n] == 0).all() and not q[rows - n - 3:rows - n].any()
+
+
 @pytest.mark.parametrize("rows,size", [(2500, 1001), (2400, 2048), (9, 1003), (300, 64)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_rows_between_rows_without_a_scale(ak, torch_cuda, rows, size, dtype):
@@ -184,6 +199,20 @@ def test_gemm(ak, torch_cuda, epi, m, n, k, pad):
 @pytest.mark.parametrize("m,n,k,pad", [(1024, 256, 16, 0), (1025, 257, 400, 0), (1500, 300, 2048, 4), (2049, 2304, 768, 0), (1200, 1003, 144, 5), (5000, 511, 128, 1)])
 def test_gemm_of_many_rows(ak, torch_cuda, epi, m, n, k, pad):
     _gemm(ak, torch_cuda, m, n, k, epi, pad)
+
+
+@pytest.mark.parametrize("n", [65600, 65601])
+def test_gemm_of_more_than_32_bits_of_results(ak, torch_cuda, n):
+    torch = torch_cuda
+    m, k, last = 70001, 32, 130
+    g = _gen(torch, n)
+    a, wt = _int8(torch, (m, k), g), _int8(torch, (n, k), g)
+    sa, sw = 0.01 + torch.rand(m, device="cuda", generator=g), (0.01 + torch.rand(n, device="cuda", generator=g)) / k
+    c = torch.full((m, n), 3.25, dtype=torch.bfloat16, device="cuda")
+    ak.ops.gemm_q8(a, sa, wt, sw, c, m, n, k, ak.EPI_STORE_BF16)
+    torch.cuda.synchronize()
+    want = (a[-last:].double() @ wt.double().t()) * sa[-last:].double()[:, None] * sw.double()
+    assert ((c[-last:].double() - want).abs() <= (2.0 ** -8 + 4 * U) * want.abs()).all()
 
 
 @pytest.mark.parametrize("m,n", [(1, 40), (130, 64), (1024, 256)])
