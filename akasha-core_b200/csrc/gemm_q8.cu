@@ -493,18 +493,24 @@ static uint32_t i8_stages(uint32_t bn, uint32_t ks, uint32_t per, uint32_t a_row
 }
 
 // The shortest of the tile widths, K splits and the pair kernel by what a launch takes, in us. Fitted to 250 measurements of 26 shapes from
-// 1 x 2304 x 768 to 2048^3 and 1500 x 1000 x 4000 (a graph of launches, weights of three sets); over these the choice loses 1.2 % on average
-// against the best of all, 10 % at most (64 x 6144 x 2048: 7.9 us with tiles of 32 columns, 7.2 with 48).
+// 1 x 2304 x 768 to 2048^3 and 1500 x 1000 x 4000 (a graph of launches, weights of three sets; over these the choice loses 1.2 % on average
+// against the best of all, 10 % at most: 64 x 6144 x 2048 7.9 us with tiles of 32 columns, 7.2 with 48), and, between tile and pair, to 291 of 200 to 5000 rows,
+// three epilogues (0.4 % on average, 31 % at most: 5000 x 1000 x 256).
 //   tile   2.1, the epilogue 0.01 a column, and per K block of b KB (activation and weight tile) 0.17 + b / 168, the rate of one TMA stream
-//          from L2; two CTAs on an SM share 121 KB/us, and every further pair of them starts anew. A split adds its exchange.
-//   pair   3.8, and 0.40 per K block of the 74 pairs.
+//          from L2; two CTAs on an SM share 121 KB/us, and every further pair of them starts anew. A split adds its exchange. With several tiles
+//          of rows, a million results takes 1.05, a third of the loads' time less; where they are added, 1.6.
+//   pair   4.4, and per turn of the 74 pairs 0.40 per K block and what of a tile's 3 us of results that does not cover.
 //   Weights come from HBM at 5.5 MB/us at most.
-static I8Plan i8_plan(uint32_t m, uint32_t n, uint32_t k) {
+static I8Plan i8_plan(uint32_t m, uint32_t n, uint32_t k, bool add) {
     const uint32_t kb = cdiv(k, I8_KB), mt = cdiv(m, I8_M), ar = i8_slot_rows(m);
     const float rows = (float)(m < I8_M ? m : I8_M), stream = (float)n * k / 5.5e6f;
     I8Plan p{};
     float best = 1e30f;
-    if (m > I8_M && n > 128) best = 3.8f + (float)cdiv64((uint64_t)cdiv(m, 2 * I8_M) * cdiv(n, I8P_BN), B200_SMS / 2) * kb * 0.40f;
+    if (m > I8_M && n > 128) {
+        const float rest = 3.0f - 0.24f * kb;
+        best = 4.4f + (float)cdiv64((uint64_t)cdiv(m, 2 * I8_M) * cdiv(n, I8P_BN), B200_SMS / 2) * (kb * 0.40f + (rest > 0.0f ? rest : 0.0f));
+    }
+    const float out = (float)m * n * (add ? 1.5f : 1.0f) / 0.95e6f;
     for (uint32_t ks = 1; ks <= 8; ks *= 2) {
         const uint32_t per = cdiv(kb, ks), unit = ks > 4 ? 32 : 16;   // a slice of bn / ks columns is whole groups of 4
         if (ks > 1 && (ks - 1) * per >= kb) break;                    // every CTA of a cluster gets work
@@ -512,8 +518,10 @@ static I8Plan i8_plan(uint32_t m, uint32_t n, uint32_t k) {
             const uint64_t ctas = (uint64_t)mt * cdiv(n, bn) * ks, turns = (ctas + 2 * B200_SMS - 1) / (2 * B200_SMS);
             if (ks > 1 && i8_stages(bn, ks, per, ar, ctas) < (per < 4 ? per : 4)) continue;   // the exchange buffer leaves no ring
             const float b = (float)(ar + bn) * I8_KB * 1e-3f, one = 0.17f + b / 168.0f, two = b / 60.5f;
-            const float load = per * (ctas <= B200_SMS ? one : (float)turns * (one > two ? one : two));
+            const float load = per * (ctas <= B200_SMS ? one : (float)turns * (one > two ? one : two) * (mt > 1 ? 1.08f : 1.0f));
             float t = 2.1f + 0.01f * bn + (float)(turns - 1) * 0.9f + (load > stream ? load + 0.15f * stream : stream + 0.15f * load);
+            const float hidden = add ? 0.0f : 0.35f * load;
+            if (mt > 1 && out > hidden) t += out - hidden;
             if (ks > 1) t += 0.8f + rows * bn * 4e-3f * (float)(ks - 1) / (float)ks / 7.9f;
             if (t < best) { best = t; p.bn = bn; p.ks = ks; }
         }
@@ -538,7 +546,7 @@ static int i8_launch_tile(cudaStream_t st, const CUtensorMap& tmA, const CUtenso
 template <int EPI>
 static int i8_launch_epi(cudaStream_t st, const void* a, const void* wt, const GemmEpi& ep, const I8Scales& sc, uint32_t m, uint32_t n, uint32_t k) {
     CUtensorMap tmA, tmB;
-    const I8Plan p = i8_plan(m, n, k);
+    const I8Plan p = i8_plan(m, n, k, EPI == AK_EPI_ADD_F32);
     if (!p.bn) {
         static bool set[64] = {};
         AK_TRY(q8_allow_smem(gemm_q8_pair_kernel<EPI>, set, I8_SMEM_PAIR));
