@@ -317,7 +317,8 @@ AK_API int ak_kv_read_q8(void* stream, const int8_t* k_pool, const int8_t* v_poo
  *   own (kv_lens counts the new tokens, which are in the cache already). Lengths are cut at 16 * max_blocks_per_seq; a query with no
  *   position to see gives zeros. block_tables int32 [rows, max_blocks_per_seq], entries past a sequence's end are not used; the positions of a
  *   block id outside the pool are left out. scale multiplies q . k.
- *   n_splits: CTAs that share a sequence, as one thread-block cluster; 0 = the library's choice, else 1 to 16.
+ *   n_splits: CTAs that share a sequence, as one thread-block cluster; 0 = the library's choice (for
+ *   sequences that fill half of their tables), else 1 to 16.
  * Sums, maxima and softmax weights are f32. A query is held as integers of 24 bits (f32) or 16 bits (bf16) of its head's largest value (one under
  * 1e-30 counts as 0); the weights of V have 22 bits, or, for bf16 with more than 4 query rows per kv head (q_len * heads / kv_heads), 11. A weight
  * times its value's scale below 2^-40 (11 bits: 2^-29) of the sequence's largest value scale may count as 0. */
