@@ -23,7 +23,7 @@
 //
 // Measured (graph of launches on three sets of inputs, cold L2): 64 sequences x 16 heads x 128, 64 to 4096 positions 90 us = 0.96 of the copy
 // bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 22.6 us = 0.73: bound by instructions there (some 210 a tile of 2176 bytes, issue
-// slots three quarters busy); 2 sequences of 60000 x 8 kv heads x 16 query rows 63 us = 0.59: few CTAs, instructions; one sequence of 300 x 5 heads
+// slots three quarters busy); 2 sequences of 60000 x 8 kv heads x 16 query rows 64 us = 0.57: few CTAs, instructions; one sequence of 300 x 5 heads
 // 5.8 us, a chain of latencies (the shortest launch takes 1.3).
 //
 // A CTA takes one (sequence, kv head, tile of queries, split); each warp has every n-th cache block of the split and a ring of cp.async
@@ -400,6 +400,13 @@ attn_decode_q8_kernel(const AqArgs a) {
             ks[b][0] = lds_f(sks); ks[b][1] = lds_f(sks + 32);
             vs[b][0] = lds_f(sks + 64); vs[b][1] = lds_f(sks + 96);
         }
+        if (!whole) {   // behind the last row's end may be anything, a NaN for a scale included: nothing of it may move a reference, or the results' last bits
+#pragma unroll
+            for (int b = 0; b < TURN; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (pos[b] + 8 * h >= lim_max) ks[b][h] = vs[b][h] = 0.0f;
+        }
         float x[TURN][NQ][2], p[TURN][NQ][2], most = -INFINITY, v_most = 0.0f;   // q . k without scales; exponents 2^..; the largest of these; of the value scales
 #pragma unroll
         for (int b = 0; b < TURN; b++) {
@@ -415,8 +422,8 @@ attn_decode_q8_kernel(const AqArgs a) {
                     most = fmaxf(most, p[b][u][h]);
                 }
         }
-        // A score more than 8 above its row's reference, or a value scale that the weights' power of two does not cover yet. (In a turn that not every
-        // row sees to its end, also by what nobody sees: the branch looks again.)
+        // A score more than 8 above its row's reference, or a value scale that the weights' power of two does not cover yet. (Also by positions that not
+        // every row sees: the branch looks again.)
         if (__any_sync(0xffffffffu, most > 8.0f || v_most >= pow2i(v_exp))) {
             float vtop = 0.0f;
 #pragma unroll
@@ -472,7 +479,7 @@ attn_decode_q8_kernel(const AqArgs a) {
                     w[b][u][h] = p[b][u][h] * f;
                 }
             }
-        if (!whole) {   // positions that a row does not see may hold anything, a NaN for a scale included
+        if (!whole) {   // positions that a row does not see
 #pragma unroll
             for (int b = 0; b < TURN; b++)
 #pragma unroll

@@ -563,6 +563,27 @@ def test_attn_values_that_are_not_finite(ak, torch_cuda):
     assert torch.equal(bad.all(-1), want) and torch.equal(bad.any(-1), want)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,q_len,heads", [(32, 1, 4), (64, 1, 2), (64, 3, 8), (96, 1, 2), (96, 5, 4), (128, 1, 2), (128, 2, 8)])
+def test_attn_bits_do_not_depend_on_what_nobody_sees(ak, torch_cuda, dtype, hd, q_len, heads):
+    """Behind a sequence's end, in the rest of its last block, lies anything: the same bits come out."""
+    torch = torch_cuda
+    dt, tdt = _dt(ak, torch, dtype)
+    lens = [500, 37, 1000, 1, 15, 333, 90, 2001, 700, 701, 702, 703, 1234, 60]
+    cache, tables, klens, blocks, mb = _attn_case(torch, lens, 2, hd, 3)
+    unseen = cache[2].isnan()
+    q = (2 * torch.randn(len(lens) * q_len, heads * hd, device="cuda", generator=_gen(torch, 1))).to(tdt)
+    outs = []
+    for k_scale, v_scale in ((float("nan"), float("nan")), (1e-3, 1e25), (1e3, 1e-25)):
+        cache[2].masked_fill_(unseen, k_scale)
+        cache[3].masked_fill_(unseen, v_scale)
+        out = torch.empty_like(q)
+        ak.ops.attn_decode_paged_q8(q, *cache, tables, klens, out, len(lens), q_len, heads, 2, hd, mb, hd ** -0.5, blocks, dtype=dt)
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
 def test_attn_far_blocks(ak, torch_cuda):
     """Offsets past 32 bits: pools of 4.3 GB each, the sequences at their ends."""
     torch = torch_cuda
