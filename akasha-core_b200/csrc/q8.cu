@@ -70,12 +70,10 @@ struct RowScale {
 };
 __device__ __forceinline__ RowScale row_scale(bool norm, float sum, float top, float inv_size, float eps) {
     const float y = norm ? top * rsqrtf(sum * inv_size + eps) : top;
-    const bool some = y >= Q8_ZERO && top >= 1e-36f;   // (127 / top would overflow)
-    float r;   // 128 / top, as in q8_scale
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top * 0.0078125f));
+    const bool some = y >= Q8_ZERO && top >= 1e-36f;   // (127 / top is below 2^127, and products h w keep 2^-30 of their largest)
     RowScale o;
     o.ok = y < INFINITY;
-    o.inv = some && o.ok ? r * 0.9921875f : 0.0f;
+    o.inv = some && o.ok ? q8_inv(top) : 0.0f;
     o.s = !o.ok ? __uint_as_float(0x7fc00000u) : some ? y * (1.0f / 127.0f) : 0.0f;
     return o;
 }

@@ -53,6 +53,8 @@ inline int q8_allow_smem(K* kernel, bool* set, uint32_t bytes, bool wide_cluster
 // Rows whose largest value is under Q8_ZERO (127 / max would overflow) are zeros, s = 0; a row with an infinity or a NaN has s = NaN
 // and q = 0, so that whatever is computed from it is NaN and nothing else is.
 constexpr float Q8_ZERO = 1e-30f;
+// 127 / top for top from 1e-37 on, in two roundings: the quarter keeps the reciprocal of the largest values out of the subnormal numbers.
+__device__ __forceinline__ float q8_inv(float top) { return __fmul_rn(__frcp_rn(top * 0.25f), 31.75f); }
 __device__ __forceinline__ void q8_scale(uint32_t top_bits, float& inv, float& s) {
     const float top = __uint_as_float(top_bits);
     float r;   // 128 / top: the factor keeps the reciprocal of the largest values away from what the approximation flushes to 0
