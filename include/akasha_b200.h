@@ -274,7 +274,8 @@ AK_API int ak_bf16_to_f32(void* stream, const void* src, float* dst, uint64_t n)
 
 /* ---- 8-bit operators (no counterpart in the reference) ----
  * A row of numbers y is held as int8 values q = rint(127 y / max|y|) in -127..127 and one f32 scale s = max|y| / 127: y ~ q s, off by at
- * most s / 2. Rows are a token's activations, an output channel's weights, or one head's key or value at one cached position. A row whose
+ * most s / 2. In f32: q = rint(y (127 (1 / max|y|))) and s = max|y| (1 / 127), each operation rounded, half-way cases to the even integer, the same
+ * for every size and alignment (under the norm y is h w here, and s is multiplied by the root). Rows are a token's activations, an output channel's weights, or one head's key or value at one cached position. A row whose
  * largest magnitude is under 1e-30 is held as zeros with s = 0 (under the norm also one whose largest h w, before the root divides it, is under
  * 1e-36); one with an infinity or a NaN (under the norm: in h w) as zeros with s = NaN, so that whatever is computed from it is NaN. A call whose
  * output (or, for the cache, key pool) lies on another device than the current one, or in memory that no

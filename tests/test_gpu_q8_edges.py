@@ -46,3 +46,63 @@ def test_norm_of_products_next_to_the_smallest(ak, torch_cuda, rows, size, offse
     assert (q[none] == 0).all() and (scales[none] == 0).all()
     # a product of the smallest kept rows may be subnormal: half a step of these, 2^-150, is 2^-30 of 1e-36 and less
     _check_rows(torch, _normed(torch, x, w, 0.0)[~none], _norm_error(size) + 2.0 ** -30, q[~none], scales[~none])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,size,offset", FORMS + [(700, 14001, 0), (130, 3, 0)])
+def test_rows_take_three_roundings(ak, torch_cuda, dtype, rows, size, offset):
+    """q = rint(y (127 (1 / max|y|))) with each of the operations rounded to f32, half-way cases to even: the same integers whatever kernel a size or an
+    alignment picks. Values of bf16 are often half-way."""
+    torch = torch_cuda
+    dt, tdt = _dt(ak, torch, dtype)
+    x = torch.randn(rows, size, device="cuda", generator=_gen(torch, rows + size)).to(tdt)
+    x = x * torch.ldexp(torch.ones(rows, 1, device="cuda"), torch.arange(rows, device="cuda")[:, None] % 200 - 80).to(tdt)
+    x[-1] = x[-1].sign() * 3.0e38        # the largest numbers
+    x = _at(torch, x, offset)
+    q, scales = torch.full((rows, size), 77, dtype=torch.int8, device="cuda"), torch.full((rows,), 7.0, device="cuda")
+    ak.ops.rmsnorm_q8(x, None, None, q, scales, rows, size, in_dtype=dt)
+    torch.cuda.synchronize()
+    y = x.float()
+    top = y.abs().amax(1, keepdim=True)
+    inv = (top * 0.25).reciprocal() * 31.75        # (the quarter: 1 / 3e38 is subnormal)
+    assert torch.equal(q.float(), torch.round(y * inv))
+    assert torch.equal(scales[:, None], top * torch.tensor(1.0 / 127.0, dtype=torch.float32, device="cuda"))
+
+
+def test_half_way_values_go_to_the_even_integer(ak, torch_cuda):
+    """max|y| = 127 times a power of two: the quotients are the values, exactly."""
+    torch = torch_cuda
+    y = torch.arange(-254, 255, device="cuda").float() / 2
+    for dtype in ("f32", "bf16"):
+        dt, tdt = _dt(ak, torch, dtype)
+        for power in (-90, -3, 0, 60):
+            x = torch.ldexp(y, torch.tensor(power, device="cuda")).to(tdt).expand(3, -1).contiguous()
+            q, scales = torch.full(x.shape, 77, dtype=torch.int8, device="cuda"), torch.full((3,), 7.0, device="cuda")
+            ak.ops.rmsnorm_q8(x, None, None, q, scales, 3, x.shape[1], in_dtype=dt)
+            torch.cuda.synchronize()
+            assert torch.equal(q.float(), torch.round(y).expand(3, -1))
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(2, 1, 32), (5, 5, 64), (6, 3, 96), (4, 2, 128)])
+def test_append_takes_three_roundings(ak, torch_cuda, heads, kv_heads, hd):
+    """The same of the cache's rows: values as they are, keys rotated with one rounding per operation; half of the values are those of bf16."""
+    torch = torch_cuda
+    tokens, blocks = 333, 30
+    g = _gen(torch, hd)
+    x = torch.randn(tokens, heads + 2 * kv_heads, hd, device="cuda", generator=g)
+    x[::2] = x[::2].bfloat16().float()
+    table = ops8._rope_table(torch, 50, hd)
+    pos = torch.randint(0, 50, (tokens,), device="cuda", generator=g, dtype=torch.int32)
+    slots = torch.randperm(blocks * 16, device="cuda", generator=g)[:tokens].to(torch.int32)
+    kp, vp, ks, vs = ops8._cache(torch, blocks, kv_heads, hd, 1)
+    q = torch.empty(tokens, heads * hd, device="cuda")
+    ak.ops.rope_kv_append_q8(x, table, 50, pos, slots, q, kp, vp, ks, vs, tokens, heads, kv_heads, hd, blocks, dtype=ak.AK_F32)
+    torch.cuda.synchronize()
+    a, b, c, s = x[..., 0::2], x[..., 1::2], table[pos.long()][:, None, :, 0], table[pos.long()][:, None, :, 1]
+    turned = torch.stack([a * c - b * s, a * s + b * c], -1).flatten(-2)
+    assert torch.equal(q.view(tokens, heads, hd), turned[:, :heads])
+    at = slots.long()
+    for pool, scales, y in ((kp, ks, turned[:, heads:heads + kv_heads]), (vp, vs, x[:, heads + kv_heads:])):
+        top = y.abs().amax(-1, keepdim=True)
+        assert torch.equal(pool[at // 16, :, at % 16].float(), torch.round(y * (top.reciprocal() * 127)))
+        assert torch.equal(scales[at // 16, :, at % 16][..., None], top * torch.tensor(1.0 / 127.0, dtype=torch.float32, device="cuda"))
