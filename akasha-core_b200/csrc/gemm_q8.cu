@@ -48,12 +48,16 @@ __device__ __forceinline__ void col_scales(const float* w, uint32_t col, uint32_
     }
 }
 
+// The sum of products to f32, times the row's and then the column's scale, every operation rounded: none of them is fused with an addition behind it, so that
+// a result has the same bits whichever way it takes to memory (the tensor memory accelerator's addition, a vector, one element).
+__device__ __forceinline__ float i8_scaled(int32_t sum, float sa, float sw) { return __fmul_rn(__fmul_rn((float)sum, sa), sw); }
+
 // One result, with the epilogue's operation; `old` is what it is added to.
 template <int EPI>
 __device__ __forceinline__ void store_one(const GemmEpi& ep, uint32_t row, uint32_t col, float v, float old) {
     const size_t at = (size_t)row * ep.ldc + col;
     if constexpr (EPI == AK_EPI_STORE_F32) reinterpret_cast<float*>(ep.c)[at] = v;
-    else if constexpr (EPI == AK_EPI_ADD_F32) reinterpret_cast<float*>(ep.c)[at] = v + old;
+    else if constexpr (EPI == AK_EPI_ADD_F32) reinterpret_cast<float*>(ep.c)[at] = __fadd_rn(v, old);
     else reinterpret_cast<bf16*>(ep.c)[at] = __float2bfloat16_rn(EPI == AK_EPI_SILU_BF16 ? epi_silu(v) : v);
 }
 // 16 columns of a warp's 32 rows where rows are not aligned for vectors (an odd pitch, the last columns): turned in shared memory (32 x 17 floats) so
@@ -184,7 +188,7 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                 tmem_ld16(tmem_base + ((quad * 32u) << 16) + c0, r);
                 tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; j++) v[j] = (float)(int32_t)r[j] * sa * sw[j];
+                for (int j = 0; j < 16; j++) v[j] = i8_scaled((int32_t)r[j], sa, sw[j]);
                 if (c0 + 16 < bn) col_scales<16>(sc.w, n0 + c0 + 16, n, vec, sw);
                 // (the ring's first 16 KB are free by now: every MMA has read its operands)
                 if (n0 + c0 + 16 <= n && (ep.ldc & 7u) == 0) epi_store16<EPI>(ep, row, row < m, n0 + c0, v, n, lane);
@@ -231,7 +235,7 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     const uint32_t col = n0 + rank * SL + j;
                     float s4[4];
                     col_scales<4>(sc.w, col, n, vec, s4);
-                    const float v[4] = {(float)acc.x * sa * s4[0], (float)acc.y * sa * s4[1], (float)acc.z * sa * s4[2], (float)acc.w * sa * s4[3]};
+                    const float v[4] = {i8_scaled(acc.x, sa, s4[0]), i8_scaled(acc.y, sa, s4[1]), i8_scaled(acc.z, sa, s4[2]), i8_scaled(acc.w, sa, s4[3])};
                     epi_store<EPI, 4>(ep, row, col, v, n);
                 }
             }
@@ -246,7 +250,7 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                         int32_t acc = 0;
                         for (uint32_t src = 0; src < ks; src++) acc += red[((size_t)src * a_rows + quad * 32 + r) * SL + c];
                         const float old = EPI == AK_EPI_ADD_F32 ? reinterpret_cast<const float*>(ep.c)[(size_t)row_i * ep.ldc + col] : 0.0f;
-                        store_one<EPI>(ep, row_i, col, (float)acc * s_row * sc.w[col], old);
+                        store_one<EPI>(ep, row_i, col, i8_scaled(acc, s_row, sc.w[col]), old);
                     }
                     for (c += 32; c >= SL; c -= SL) r++;
                 }
@@ -406,7 +410,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[tc & 1u]), 0));
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = (float)(int32_t)r[j] * sa * sw[j];
+                for (int j = 0; j < 32; j++) v[j] = i8_scaled((int32_t)r[j], sa, sw[j]);
                 if (c0 + 32 < (uint32_t)I8P_EPI_COLS) col_scales<32>(sc.w, n0 + c0 + 32, n, vec, sw);
                 const uint32_t col = n0 + (OUT_BF16 ? (c0 & ~32u) : c0);   // first column of the staged piece
                 // a store is clipped at n in whole 16-byte units only: a ragged last piece is stored from registers

@@ -106,3 +106,28 @@ def test_append_takes_three_roundings(ak, torch_cuda, heads, kv_heads, hd):
         top = y.abs().amax(-1, keepdim=True)
         assert torch.equal(pool[at // 16, :, at % 16].float(), torch.round(y * (top.reciprocal() * 127)))
         assert torch.equal(scales[at // 16, :, at % 16][..., None], top * torch.tensor(1.0 / 127.0, dtype=torch.float32, device="cuda"))
+
+
+# ------------------------------------------------------------------ product
+@pytest.mark.parametrize("epi", [0, 1, 2, 3])
+@pytest.mark.parametrize("n,k,pad", [(768, 2304, 0), (2048, 2048, 0), (777, 1024, 0), (300, 4096, 5), (1002, 2048, 0)])
+def test_product_rows_do_not_depend_on_the_batch(ak, torch_cuda, epi, n, k, pad):
+    """A row alone, in decode batches, in prompts: the same bits with every epilogue and any pitch, whatever kernel and split it ran on."""
+    torch = torch_cuda
+    g = _gen(torch, n + k)
+    most, ld = 3000, n + pad
+    a, wt = _int8(torch, (most, k), g), _int8(torch, (n, k), g)
+    sa, sw = 0.01 + torch.rand(most, device="cuda", generator=g), (0.01 + torch.rand(n, device="cuda", generator=g)) / k
+    start = torch.randn(most, ld, device="cuda", generator=g).to(torch.float32 if epi < 2 else torch.bfloat16)
+
+    def product(m):
+        c = start[:m].clone()
+        ak.ops.gemm_q8(a[:m], sa[:m], wt, sw, c, m, n, k, epi, ldc=ld)
+        return c
+
+    full = product(most)
+    for m in (1, 3, 8, 17, 64, 100, 128, 200, 500, 1000, 2048):
+        assert torch.equal(product(m), full[:m]), m
+    if epi < 2:    # the sum to f32, two products, and the addition, each rounded
+        y = (a.double() @ wt.double().t()).float() * sa[:, None] * sw
+        assert torch.equal(full[:, :n], start[:, :n] + y if epi == 1 else y)
