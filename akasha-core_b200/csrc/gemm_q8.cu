@@ -219,7 +219,7 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     }
                 }
             }
-            // a CTA leaves only after it has received everything addressed to it, so nobody writes into one that is gone
+            // a CTA leaves after it has received everything addressed to it, or through cluster_leave_after_failure: nobody writes into one that is gone
             bool landed = mbar_wait(&xch_bar, 0);
             if (!landed && lane == 0) atomicExch(&fail_flag, 6u);
             got = __all_sync(0xffffffffu, landed);
@@ -260,6 +260,7 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && fail_flag) atomicExch(&g_gemm_q8_status, fail_flag);
+    if (SPLIT && fail_flag) cluster_leave_after_failure(&xch_bar);
     if (warp == 1) {
         __syncwarp();
         tmem_dealloc(tmem_base, tmem_cols);

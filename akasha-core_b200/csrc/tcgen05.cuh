@@ -98,7 +98,13 @@ __device__ __forceinline__ void st_async_v4(uint32_t dst_cluster_addr, uint32_t 
                  "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar_cluster_addr)
                  : "memory");
 }
-
+// The way out of a CTA whose cluster exchanges slices by st_async_v4 and that has given up a wait, for all of its threads: peers that have not may still send it
+// theirs. It stays until every thread of the cluster has left or come here as well (a barrier does not wait for threads that have left), which is to say
+// has sent what it ever will, and then, a bounded time, for what is on its way. A CTA that has received everything leaves without.
+__device__ __forceinline__ void cluster_leave_after_failure(uint64_t* xch_bar) {
+    cluster_sync_all();
+    mbar_wait(xch_bar, 0);
+}
 
 // ---- two CTAs of a cluster on one tile (cta_group::2)
 __device__ __forceinline__ uint32_t cluster_ctarank() {
