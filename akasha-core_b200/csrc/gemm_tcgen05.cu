@@ -261,8 +261,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
         }
         // Every peer's slices for this CTA have landed when the exchange barrier's byte count is met: no cluster-wide
-        // barrier (0.75 us). A CTA leaves only after it has received everything addressed to it, so nobody writes
-        // into a CTA that is gone.
+        // barrier (0.75 us). A CTA leaves after it has received everything addressed to it, or through
+        // cluster_leave_after_failure, so nobody writes into a CTA that is gone.
         if (warp >= 2 && got) {
             bool landed = mbar_wait(&xch_bar, 0);
             if (!landed && lane == 0) atomicExch(&fail_flag, 6u);
@@ -291,6 +291,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && fail_flag) atomicExch(&g_gemm_status, fail_flag);
+    if (SPLIT && fail_flag) cluster_leave_after_failure(&xch_bar);
     if (warp == 1) {
         __syncwarp();
         tmem_dealloc(tmem_base, tmem_cols);
