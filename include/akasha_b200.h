@@ -284,6 +284,8 @@ AK_API int ak_bf16_to_f32(void* stream, const void* src, float* dst, uint64_t n)
 
 /* RMS norm with the residual's addition and an 8-bit result:
  *   h = x + residual (residual != NULL: f32 x only; h is written back to x), y = h * rsqrt(mean(h^2) + eps) * w per row, q and scales as above.
+ *   The squares are added in f32: a row whose sum of h^2 is beyond f32's largest number (values of about 1e18 and more) or whose mean(h^2) + eps is under
+ *   1e-36 gives zeros with s = NaN; one of zeros gives zeros with s = 0 whatever eps is.
  *   w == NULL: y = h, the rows are quantised as they are (weights [n,k] for ak_gemm_q8, activations behind SiLU or attention).
  * x [seq_len, size] f32 or bf16 (in_dtype); residual f32, w f32 [size]; q int8 [seq_len, size]; scales f32 [seq_len]. Any size;
  * rows of up to 32768 values (sizes that are no multiple of 16 bytes of x: 14000) are read once if x, residual and w are 16-byte aligned and q to the bytes of 16 bytes of x (4, bf16 8),

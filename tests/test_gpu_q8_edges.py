@@ -131,3 +131,39 @@ def test_product_rows_do_not_depend_on_the_batch(ak, torch_cuda, epi, n, k, pad)
     if epi < 2:    # the sum to f32, two products, and the addition, each rounded
         y = (a.double() @ wt.double().t()).float() * sa[:, None] * sw
         assert torch.equal(full[:, :n], start[:, :n] + y if epi == 1 else y)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,size,offset", FORMS + [(600, 200, 1)])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 1e-5])
+def test_norm_at_the_ends_of_its_range(ak, torch_cuda, dtype, rows, size, offset, residual, eps):
+    """Mean squares from 1e-36 on up to sums of f32's largest number are ordinary. Outside (values of 1e20, or 1e-20 without eps) the scale is NaN, not that of
+    another row or a zero, and nothing else of the call is. Zeros are zeros, without eps too."""
+    torch = torch_cuda
+    if residual and dtype == "bf16":
+        pytest.skip("a residual is added to f32 rows only")
+    dt, tdt = _dt(ak, torch, dtype)
+    kind = torch.arange(rows, device="cuda") % 8
+    power = torch.tensor([0, 66, -83, 120, 0, -66, 54, -56], device="cuda")[kind]       # 2^66 = 7e19, 2^-83 = 1e-25, 2^-56 = 1.4e-17
+    g = _gen(torch, size + rows)
+    x = torch.randn(rows, size, device="cuda", generator=g)
+    x[kind == 4] = 0
+    res = 0.5 * x.flip(1) if residual else None
+    x = torch.ldexp(x, power[:, None]).to(tdt)
+    w = 1 + 0.2 * torch.randn(size, device="cuda", generator=g)
+    if res is not None:
+        res = _at(torch, torch.ldexp(res, power[:, None]), offset)
+    x, w = _at(torch, x, offset), _at(torch, w, offset)
+    h = x + res if res is not None else x.clone()
+    q, scales = torch.full((rows, size), 77, dtype=torch.int8, device="cuda"), torch.full((rows,), 7.0, device="cuda")
+    ak.ops.rmsnorm_q8(x, res, w, q, scales, rows, size, eps, in_dtype=dt)
+    torch.cuda.synchronize()
+    assert torch.equal(x, h)
+    none, lost = kind == 4, (kind == 1) | (kind == 3)
+    if eps == 0:
+        lost |= (kind == 2) | (kind == 5)
+    assert (q[none] == 0).all() and (scales[none] == 0).all()
+    assert (q[lost] == 0).all() and scales[lost].isnan().all()
+    kept = ~(none | lost)
+    _check_rows(torch, _normed(torch, h, w, eps)[kept], _norm_error(size), q[kept], scales[kept])
