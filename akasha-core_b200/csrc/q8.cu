@@ -196,7 +196,7 @@ norm_q8_ring_kernel(T* __restrict__ x, const float* __restrict__ residual, const
     }
     const uint32_t my = smem_u32(ring) + t * 16;
     const size_t stride = (size_t)step * size, off0 = (size_t)blockIdx.x * size - shift + V * t;
-    // (a partial group is read whole, with neighbouring rows' values that are dropped, but not past the last row)
+    // (a partial group is read whole, with neighbouring rows' values that are dropped, but not past the last row: the one before it has V values behind it)
     auto ask = [&](uint32_t row, size_t off, uint32_t half) {
         if (row < rows) {
 #pragma unroll
@@ -285,7 +285,7 @@ norm_q8_ring_kernel(T* __restrict__ x, const float* __restrict__ residual, const
     }
 }
 
-// Rows that do not fit the registers of a block, and buffers that are not aligned for vectors: a block per row, two passes over it (the second reads what
+// Rows that do not fit the registers of a block, rows shorter than a vector, and buffers that are not aligned for vectors: a block per row, two passes over it (the second reads what
 // the first wrote back).
 template <typename T>
 __global__ void __launch_bounds__(1024)
@@ -320,8 +320,8 @@ static int norm_q8(cudaStream_t st, T* x, const float* residual, const float* w,
     const uint32_t groups = cdiv(size, V) + (size % V ? 1 : 0);   // of a row, at most
     const float inv_size = 1.0f / (float)size;
     const bool vectors = q8_aligned(x, 16) && q8_aligned(residual, 16) && q8_aligned(q, V) && q8_aligned(w, 16);
-    if (!vectors)
-        return launch_k(norm_q8_any_kernel<T>, dim3(rows), dim3(512), 0, st, NO_CLUSTER, x, residual, w, q, scales, size, inv_size, eps);
+    if (!vectors || size < V)   // (rows shorter than a vector: those of several rows would reach over the end of the buffer)
+        return launch_k(norm_q8_any_kernel<T>, dim3(rows), dim3(size < V ? 32 : 512), 0, st, NO_CLUSTER, x, residual, w, q, scales, size, inv_size, eps);
     const bool few = rows <= 2 * B200_SMS;   // latency: as many threads to a row as there are vectors
     const bool odd = size % V != 0;
     // The ring: any odd size; with weights, rows of more than 24 values a lane of one warp (16384 x 1024 f32 14.9 us, in the other kernel 17.4, but 768 12.5

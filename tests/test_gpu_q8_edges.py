@@ -167,3 +167,25 @@ def test_norm_at_the_ends_of_its_range(ak, torch_cuda, dtype, rows, size, offset
     assert (q[lost] == 0).all() and scales[lost].isnan().all()
     kept = ~(none | lost)
     _check_rows(torch, _normed(torch, h, w, eps)[kept], _norm_error(size), q[kept], scales[kept])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("size", [1, 2, 3, 5, 6, 7, 9, 11])
+def test_norm_of_rows_about_as_short_as_a_vector(ak, torch_cuda, dtype, residual, size):
+    """Several rows to 16 bytes: a row's vectors would reach over its neighbours, and over the end of the buffer for more rows than the last."""
+    torch = torch_cuda
+    if residual and dtype == "bf16":
+        pytest.skip("a residual is added to f32 rows only")
+    dt, tdt = _dt(ak, torch, dtype)
+    for rows in (1, 2, 3, 4, 5, 7, 9, 150, 1201):
+        g = _gen(torch, 10 * rows + size)
+        x = torch.randn(rows, size, device="cuda", generator=g).to(tdt)
+        res = torch.randn(rows, size, device="cuda", generator=g) if residual else None
+        w = 1 + 0.2 * torch.randn(size, device="cuda", generator=g)
+        h = x + res if residual else x.clone()
+        q, scales = torch.full((rows, size), 77, dtype=torch.int8, device="cuda"), torch.full((rows,), 7.0, device="cuda")
+        ak.ops.rmsnorm_q8(x, res, w, q, scales, rows, size, in_dtype=dt)
+        torch.cuda.synchronize()
+        assert torch.equal(x, h)
+        _check_rows(torch, _normed(torch, h, w, 1e-5), _norm_error(size), q, scales)
