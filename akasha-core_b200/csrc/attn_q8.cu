@@ -18,8 +18,8 @@
 // registers instead of 280 and 122, and 64 x 16 heads x 2048 positions x 128 113 us instead of 86.
 //
 // Weights are 2^(s - m) with a reference m that follows the running maximum only when a score is more than 8 above it: up to then weights
-// grow to 2^8, which f16 has room for (they are scaled by a power of two, below 2^13, that follows the largest value scale met so far), and no
-// reduction over the lanes stands between the two products.
+// grow to 2^8, which f16 has room for (they are scaled by a power of two, below 2^13, that follows the largest value scale that the query has met so
+// far), and no reduction over the lanes stands between the two products.
 //
 // Measured (graph of launches on three sets of inputs, cold L2): 64 sequences x 16 heads x 128, 64 to 4096 positions 90 us = 0.96 of the copy
 // bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 22.6 us = 0.73: bound by instructions there (some 210 a tile of 2176 bytes, issue
@@ -347,10 +347,12 @@ attn_decode_q8_kernel(const AqArgs a) {
     }
 
     float m_ref[NQ], l_run[NQ];
+    int v_exp[NQ];   // a query's weights are p * vs * 2^(5 - v_exp) with vs < 2^v_exp for every finite value scale that it has seen so far
 #pragma unroll
     for (int u = 0; u < NQ; u++) {
-        const bool sees = lim[u] > 0;   // one that does not never asks for a reference
+        const bool sees = lim[u] > 0;   // one that does not never asks for a reference, or a power of two
         m_ref[u] = sees ? -INFINITY : 0.0f;
+        v_exp[u] = sees ? -110 : 127;
         if (!sees) row_scale[u] = 0.0f;
         l_run[u] = 0.0f;
     }
@@ -361,7 +363,6 @@ attn_decode_q8_kernel(const AqArgs a) {
     for (int u = 0; u < NP; u++)
 #pragma unroll
         for (int j = 0; j < MT; j++) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.0f;
-    int v_exp = -110;   // weights are p * vs * 2^(5 - v_exp) with vs < 2^v_exp for every finite value scale so far
 
     for (uint32_t i = 0; i < mine; i += TURN) {
 #pragma unroll
@@ -422,33 +423,34 @@ attn_decode_q8_kernel(const AqArgs a) {
                     most = fmaxf(most, p[b][u][h]);
                 }
         }
-        // A score more than 8 above its row's reference, or a value scale that the weights' power of two does not cover yet. (Also by positions that not
-        // every row sees: the branch looks again.)
-        if (__any_sync(0xffffffffu, most > 8.0f || v_most >= pow2i(v_exp))) {
-            float vtop = 0.0f;
+        // A score more than 8 above its row's reference, or a value scale that a row's power of two does not cover yet. (Also by positions that not
+        // every row sees: the branch looks again, so that what a row does not see neither moves its reference nor takes bits from its weights.)
+        int v_least = v_exp[0];
 #pragma unroll
-            for (int b = 0; b < TURN; b++)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (pos[b] + 8 * h < lim_max && fabsf(vs[b][h]) < INFINITY) vtop = fmaxf(vtop, fabsf(vs[b][h]));
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
-            const int ve = (int)(__float_as_uint(vtop) >> 23) - 126;   // vtop < 2^ve
-            float regrade = 1.0f;
-            if (ve > v_exp) { regrade = ve - v_exp > 120 ? 0.0f : pow2i(v_exp - ve); v_exp = ve; }   // the same in every lane
+        for (int u = 1; u < NQ; u++) v_least = min(v_least, v_exp[u]);
+        if (__any_sync(0xffffffffu, most > 8.0f || v_most >= pow2i(v_least))) {
             float corr[NQ];
 #pragma unroll
             for (int u = 0; u < NQ; u++) {
-                float mb = -INFINITY;
+                float mb = -INFINITY, vtop = 0.0f;
 #pragma unroll
                 for (int b = 0; b < TURN; b++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         p[b][u][h] = x[b][u][h] * (row_scale[u] * ks[b][h]);
-                        if (pos[b] + 8 * h < lim[u]) mb = fmaxf(mb, p[b][u][h]);
+                        if (pos[b] + 8 * h < lim[u]) {
+                            mb = fmaxf(mb, p[b][u][h]);
+                            if (fabsf(vs[b][h]) < INFINITY) vtop = fmaxf(vtop, fabsf(vs[b][h]));
+                        }
                     }
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+                for (int o = 4; o < 32; o <<= 1) {
+                    mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+                    vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
+                }
+                const int ve = (int)(__float_as_uint(vtop) >> 23) - 126;   // vtop < 2^ve
+                float regrade = 1.0f;
+                if (ve > v_exp[u]) { regrade = ve - v_exp[u] > 120 ? 0.0f : pow2i(v_exp[u] - ve); v_exp[u] = ve; }
                 const float m_new = fmaxf(m_ref[u], mb);
                 corr[u] = m_new == -INFINITY ? 1.0f : ex2(m_ref[u] - m_new);
                 m_ref[u] = m_new;
@@ -466,19 +468,18 @@ attn_decode_q8_kernel(const AqArgs a) {
                 for (int j = 0; j < MT; j++) { acc[u][j][0] *= c0; acc[u][j][1] *= c1; acc[u][j][2] *= c0; acc[u][j][3] *= c1; }
             }
         }
-        const float vf = pow2i(5 - v_exp);
-        float w[TURN][NQ][2];
+        float w[TURN][NQ][2], vf[NQ];
+#pragma unroll
+        for (int u = 0; u < NQ; u++) vf[u] = pow2i(5 - v_exp[u]);
 #pragma unroll
         for (int b = 0; b < TURN; b++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float f = vs[b][h] * vf;
+            for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int u = 0; u < NQ; u++) {
                     p[b][u][h] = ex2(p[b][u][h]);
-                    w[b][u][h] = p[b][u][h] * f;
+                    w[b][u][h] = p[b][u][h] * (vs[b][h] * vf[u]);
                 }
-            }
         if (!whole) {   // positions that a row does not see
 #pragma unroll
             for (int b = 0; b < TURN; b++)
@@ -542,7 +543,9 @@ attn_decode_q8_kernel(const AqArgs a) {
     __syncthreads();   // every warp is done with its ring
     float* part = reinterpret_cast<float*>(smem);
     {
-        const float un = pow2i(v_exp - 5);
+        float un[NQ];
+#pragma unroll
+        for (int u = 0; u < NQ; u++) un[u] = pow2i(v_exp[u] - 5);
         float* wp = part + (size_t)warp * ROWS * HD + (HD / 8) * g;
         // rows g and g + 8 of tile j are values 2j and 2j + 1 of the lane's HD / 8, columns 2t and 2t + 1 the parts of a query or two queries
 #pragma unroll
@@ -551,10 +554,10 @@ attn_decode_q8_kernel(const AqArgs a) {
             for (int j = 0; j < MT; j++) {
                 if constexpr (TWO) {
                     *reinterpret_cast<float2*>(wp + (4 * u + t) * HD + 2 * j) =
-                        make_float2(fmaf(acc[u][j][1], 1.0f / REST, acc[u][j][0]) * un, fmaf(acc[u][j][3], 1.0f / REST, acc[u][j][2]) * un);
+                        make_float2(fmaf(acc[u][j][1], 1.0f / REST, acc[u][j][0]) * un[u], fmaf(acc[u][j][3], 1.0f / REST, acc[u][j][2]) * un[u]);
                 } else {
-                    *reinterpret_cast<float2*>(wp + (8 * u + t) * HD + 2 * j) = make_float2(acc[u][j][0] * un, acc[u][j][2] * un);
-                    *reinterpret_cast<float2*>(wp + (8 * u + 4 + t) * HD + 2 * j) = make_float2(acc[u][j][1] * un, acc[u][j][3] * un);
+                    *reinterpret_cast<float2*>(wp + (8 * u + t) * HD + 2 * j) = make_float2(acc[u][j][0] * un[(2 * u) % NQ], acc[u][j][2] * un[(2 * u) % NQ]);
+                    *reinterpret_cast<float2*>(wp + (8 * u + 4 + t) * HD + 2 * j) = make_float2(acc[u][j][1] * un[(2 * u + 1) % NQ], acc[u][j][3] * un[(2 * u + 1) % NQ]);
                 }
             }
     }

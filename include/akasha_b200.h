@@ -324,7 +324,7 @@ AK_API int ak_kv_read_q8(void* stream, const int8_t* k_pool, const int8_t* v_poo
  *   sequences that fill half of their tables), else 1 to 16.
  * Sums, maxima and softmax weights are f32. A query is held as integers of 24 bits (f32) or 16 bits (bf16) of its head's largest value (one under
  * 1e-30 counts as 0); the weights of V have 22 bits, or, for bf16 with more than 4 query rows per kv head (q_len * heads / kv_heads), 11. A weight
- * times its value's scale below 2^-40 (11 bits: 2^-29) of the sequence's largest value scale may count as 0. */
+ * times its value's scale below 2^-40 (11 bits: 2^-29) of the largest value scale that the query sees may count as 0. */
 typedef struct ak_attn_q8_params {
     uint32_t rows, q_len, heads, kv_heads, head_dim, block_size, max_blocks_per_seq;
     float scale;

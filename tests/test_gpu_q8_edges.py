@@ -189,3 +189,24 @@ def test_norm_of_rows_about_as_short_as_a_vector(ak, torch_cuda, dtype, residual
         torch.cuda.synchronize()
         assert torch.equal(x, h)
         _check_rows(torch, _normed(torch, h, w, 1e-5), _norm_error(size), q, scales)
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("dtype,q_len,heads,kv_heads,power", [("bf16", 6, 2, 2, 30), ("bf16", 8, 4, 2, 60), ("bf16", 2, 4, 2, 60), ("f32", 2, 2, 2, 60),
+                                                              ("f32", 7, 2, 1, 60)])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("n_splits", [1, 2])
+def test_attn_value_that_a_later_token_brings(ak, torch_cuda, dtype, q_len, heads, kv_heads, hd, power, n_splits):
+    """The newest token's value is 2^power times the others: the queries before it do not see it, and their results are as without it."""
+    torch = torch_cuda
+    dt, tdt = _dt(ak, torch, dtype)
+    lens = [q_len, 13, 16, 31, 200]
+    cache, tables, klens, blocks, mb = ops8._attn_case(torch, lens, kv_heads, hd, 5)
+    q = torch.randn(len(lens) * q_len, heads * hd, device="cuda", generator=_gen(torch, 2)).to(tdt)
+    for r, n in enumerate(lens):
+        cache[3][tables[r, (n - 1) // 16].long(), :, (n - 1) % 16] *= 2.0 ** power
+    out = torch.full_like(q, 7.0)
+    ak.ops.attn_decode_paged_q8(q, *cache, tables, klens, out, len(lens), q_len, heads, kv_heads, hd, mb, hd ** -0.5, blocks, dtype=dt, n_splits=n_splits)
+    torch.cuda.synchronize()
+    ops8._attn_check(torch, out.view(len(lens), q_len, -1)[:, :q_len - 1].contiguous(), q.view(len(lens), q_len, -1)[:, :q_len - 1].contiguous(), cache, tables,
+                     [n - 1 for n in lens], q_len - 1, heads, kv_heads, hd, hd ** -0.5, dtype, blocks)
