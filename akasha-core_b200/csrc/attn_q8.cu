@@ -3,28 +3,33 @@
 //   o_r = sum_j softmax_j(scale * ks_j (q_r . k_j)) vs_j v_j,   j < limit_r = kv_len - q_len + i + 1 for query i of its sequence
 //
 // k_j, v_j are int8 rows, ks_j, vs_j their f32 scales. One pass over the cache with the running maximum and sum of the softmax; the
-// bytes of the cache are read once and bound the kernel (132 bytes per position and kv head at head size 64, 264 at 128).
+// bytes of the cache are read once and bound the kernel (136 bytes per position and kv head at head size 64, 264 at 128).
 //
-// Decode has one query per (sequence, head), a group of heads or a few drafted tokens at most 16 or so: tcgen05, whose smallest tile is 64
-// rows of one K, has nothing to work with, and mma.sync takes the cache as its 16-row operand, the queries as the 8-column one. A column pair
-// is one query in two parts, so that the 8 columns are 4 queries:
+// Decode has one query per (sequence, head), a group of heads or a few drafted tokens at most 16 or so. mma.sync takes the cache as its 16-row operand and
+// the queries as the 8-column one, which with one query per kv head is enough for the bytes (0.96). Groups would fill a tcgen05 tile, 128 positions
+// by the digits of 16 queries, with each score in a register once; that form is not built, and instructions hold 16 query rows at 0.57 of the bytes.
+// A column pair is one query in two parts, so that the 8 columns are 4 queries:
 //   S^T = K q   m16n8k32 on int8 as it lies in the cache. A query is held as integers X = rint(q F), F = 127 * 256^(D - 1) / max|q|, in
 //               D signed base-256 digits: 2 for bf16 (16 bits of the head's largest value), 3 for f32 (24 bits). Sums of digits are exact.
 //   O^T = V p   m16n8k16 on f16, in which int8 is exact (1024 + 128 + v is put together by a byte permute and 1152 taken off). A weight
 //               w = p vs is its leading f16 part and what is left of it, times 2^11 (22 bits together, TWO), or, for bf16 results and more than 4 query
 //               rows, the leading part alone (11 bits; the result has 8) with two queries to a column pair.
+// What the fewer bits buy: three digits for bf16 too took 1 to 10 % more time (64 x 16 x 128 77.0 us instead of 76.0, 64 x 12 x 64 up to 512 positions 11.6
+// instead of 10.5), weights in two parts for 16 query rows 115 us instead of 69. In 64 x 16 x 128 bf16 results differ from those of f32 arithmetic by 3.8e-4 (by
+// neighbouring bf16 numbers; 5e-5 with three digits), in 16 query rows by 8e-4 (4.5e-4 with weights in two parts); against 64 bits, whose distance is the
+// results' own rounding, all of them are off by 1.7e-3.
 // Scores come out with lanes holding positions g, g + 8 of one query, and turn into the second product's operand by a transposition of 8 x 8
 // blocks (movmatrix). With the queries as the 16-row operand of f16 products (and keys converted like values) a tile took 370 instructions and 168
-// registers instead of 280 and 122, and 64 x 16 heads x 2048 positions x 128 113 us instead of 86.
+// registers instead of 280 and 117, and 64 x 16 heads x 2048 positions x 128 113 us instead of 86.
 //
 // Weights are 2^(s - m) with a reference m that follows the running maximum only when a score is more than 8 above it: up to then weights
 // grow to 2^8, which f16 has room for (they are scaled by a power of two, below 2^13, that follows the largest value scale that the query has met so
 // far), and no reduction over the lanes stands between the two products.
 //
 // Measured (graph of launches on three sets of inputs, cold L2): 64 sequences x 16 heads x 128, 64 to 4096 positions 90 us = 0.96 of the copy
-// bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 22.6 us = 0.73: bound by instructions there (some 210 a tile of 2176 bytes, issue
+// bandwidth, 2048 each 86 to 91 us; 64 x 12 heads x 64 x 1024, f32 23.4 us = 0.70: bound by instructions there (some 210 a tile of 2176 bytes, issue
 // slots three quarters busy); 2 sequences of 60000 x 8 kv heads x 16 query rows 64 us = 0.57: few CTAs, instructions; one sequence of 300 x 5 heads
-// 5.8 us, a chain of latencies (the shortest launch takes 1.3).
+// 5.7 us, a chain of latencies (the shortest launch takes 1.3).
 //
 // A CTA takes one (sequence, kv head, tile of queries, split); each warp has every n-th cache block of the split and a ring of cp.async
 // stages of its own, no barrier in the loop. The warps' results are merged in shared memory and the splits', which are the CTAs of one
@@ -677,8 +682,11 @@ template <typename T, int HD, int NQ, bool TWO> struct AqForm {
 // 60000 positions: a wave of k CTAs on an SM takes 5 (clusters 6 and 0.06 for every CTA), and for each of a warp's tiles 0.2 + 0.002 HD times k
 // (1.15 for one alone: latency), or what its bytes take at 6.5 MB/us (once for all tiles of queries). Clusters share SMs before all are taken: `alone`
 // keeps a second CTA off an SM where all clusters find room like that. Measured whole and in what it picks: 1 x 12 heads x 64 x 4000 18.3 and
-// 8.4 us (8), 2 x 5 x 32 x 9000 9.0 (9), 5 x 8 kv heads x 128 x 30000 120 and 53 (3; 60 in 4), 24 x 8 x 128 x 6000 52 whole, 63 in 2. Over the 90 shapes
+// 8.4 us (8), 2 x 5 x 32 x 9000 9.0 (9), 5 x 8 kv heads x 128 x 30000 120 and 53 (3; 60 in 4), 24 x 8 x 128 x 6000 52 whole, 63 in 2. Over 108 shapes
 // it is 4 % from the best number on average, 19 % at most (4 x 12 x 64 x 8000).
+// Tables much wider than the sequences cost: 100 positions each in tables of 4096 and more instead of 112, 1 x 12 heads x 64 6.8 us instead of 4.9 and
+// 4 x 12 7.9 instead of 5.0 (splits without work), 64 x 12 12.3 instead of 6.6 (8 warps instead of 4); 1000 positions 64 x 12 22.6 instead of 18.8. The
+// lengths are on the device, where a launch cannot be shaped by them.
 template <typename F, int HD>
 static int aq_plan(uint64_t units, uint32_t q_tiles, uint32_t max_blocks, uint32_t& warps, uint32_t& n_splits, bool& alone) {
     const uint32_t cap = F::C::CTAS * B200_SMS;   // CTAs of 8 warps on all SMs

@@ -271,7 +271,8 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 // Measured (graph of launches): 16384 x 8192 x 2048 184 us = 2990 TOPS with bf16 results, 192 with SiLU, 4001 x 2048 x 8192 added to f32 50 us (128 tiles
 // are two turns of 74 pairs, the second one not full); the tensor pipe is busy for 75 % of the cycles, and the power limit takes
 // a fifth of the clock in longer runs. What feeds it is the L2: a K block of 64 KB takes a pair 0.39 us, its MMAs 0.27. Below K = 1024 the results
-// bound it, 3 us a tile (16 epilogue warps and five stages instead of 8 and six: the same there, 4 % slower for long K).
+// bound it, 3 us a tile (16 epilogue warps and five stages instead of 8 and six: the same there, 4 % slower for long K): 8000 x 8008 x 1024 bf16 62 us, 0.63 of
+// the rate. With 168 registers, 32 of them the columns' scales, the epilogue of bf16 results without an activation spills 4 (16 bytes stored, 44 loaded).
 //
 // A cluster of two CTAs walks over [256 x 256] tiles: each stages its 128 rows of A and its half (128 rows) of the weight tile per K block, the
 // leader issues MMAs of 256 x 256 x 32 that read both CTAs' shared memory, rows 0-127 accumulate in its TMEM and rows 128-255 in the peer's.
@@ -499,8 +500,8 @@ static uint32_t i8_stages(uint32_t bn, uint32_t ks, uint32_t per, uint32_t a_row
 
 // The shortest of the tile widths, K splits and the pair kernel by what a launch takes, in us. Fitted to 250 measurements of 26 shapes from
 // 1 x 2304 x 768 to 2048^3 and 1500 x 1000 x 4000 (a graph of launches, weights of three sets; over these the choice loses 1.2 % on average
-// against the best of all, 10 % at most: 64 x 6144 x 2048 7.9 us with tiles of 32 columns, 7.2 with 48), and, between tile and pair, to 291 of 200 to 5000 rows,
-// three epilogues (0.4 % on average, 31 % at most: 5000 x 1000 x 256).
+// against the best of all, 10 % at most: 64 x 6144 x 2048 7.9 us with tiles of 32 columns, 7.2 with 48; over 80 further shapes of 1 to 128 rows 2 % and 17 %),
+// and, between tile and pair, to 291 of 200 to 5000 rows, three epilogues (0.4 % on average, 31 % at most: 5000 x 1000 x 256).
 //   tile   2.1, the epilogue 0.01 a column, and per K block of b KB (activation and weight tile) 0.17 + b / 168, the rate of one TMA stream
 //          from L2; two CTAs on an SM share 121 KB/us, and every further pair of them starts anew. A split adds its exchange. With several tiles
 //          of rows, a million results takes 1.05, a third of the loads' time less; where they are added, 1.6.

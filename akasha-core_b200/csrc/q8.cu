@@ -22,9 +22,10 @@ int q8_check_here(const void* p, const char* who) {
 // together, in one pass and with one exchange between the row's threads. A row lives in their registers from then on: every input byte is read
 // once, every output byte written once. `tpr` threads share a row.
 //
-// What bounds it: the bytes (with a residual 1.0 of the copy bandwidth, 16384 x 2048 f32 26.8 us = 0.96, 4001 x 8192 26.0 = 0.96, in the
-// ring), and instructions where these are few (4001 x 8192 bf16 with weights 20.8 us = 0.72, rows of 2047 39.6 us = 0.65). With y itself and two
-// reductions, one after the other: 31, 38, 26.6 and 50 us.
+// What bounds it: the bytes (with a residual 1.0 of the copy bandwidth, 16384 x 2048 f32 26.5 us = 0.97, 4001 x 8192 26.2 = 0.96, in the
+// ring), and instructions where these are few (4001 x 8192 bf16 with weights 21.5 us = 0.70, rows of 2047 39.7 us = 0.65). With y itself and two
+// reductions, one after the other: 31, 38, 26.6 and 50 us. Of these 0.1 to 0.5 us (32768 x 320 f32 1.2 of 11.9) are the exact reciprocal's and the
+// rounded products', see q8_scale.
 template <typename T> struct Q8Vec {
     static constexpr int V = 16 / sizeof(T);   // values of a group: a 16-byte load
     static __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
@@ -324,7 +325,7 @@ static int norm_q8(cudaStream_t st, T* x, const float* residual, const float* w,
         return launch_k(norm_q8_any_kernel<T>, dim3(rows), dim3(size < V ? 32 : 512), 0, st, NO_CLUSTER, x, residual, w, q, scales, size, inv_size, eps);
     const bool few = rows <= 2 * B200_SMS;   // latency: as many threads to a row as there are vectors
     const bool odd = size % V != 0;
-    // The ring: any odd size; with weights, rows of more than 24 values a lane of one warp (16384 x 1024 f32 14.9 us, in the other kernel 17.4, but 768 12.5
+    // The ring: any odd size; with weights, rows of more than 24 values a lane of one warp (16384 x 1024 f32 14.6 us, in the other kernel 17.4, but 768 12.5
     // and 12.3), enough of them to keep the resident blocks busy (1000 x 4096 f32 4.3 and 4.1). A residual or no weights leave nothing
     // to keep, and then blocks that come and go are as good or better (16384 x 2048 f32 with a residual 65 us, 72 in the ring).
     if (odd || (w && !residual && rows >= 16 * B200_SMS && size > 768)) {
@@ -395,7 +396,7 @@ static int norm_q8(cudaStream_t st, T* x, const float* residual, const float* w,
 // and are dealt out in turns of one row a group of lanes.
 //
 // With 4 values a lane the hundred instructions that a row takes besides its bytes (addresses, scale, shuffles) were the bound: 16001 tokens, bf16, 12 + 2 x
-// 12 heads of 64 58 us then, 35 now (0.86 of the copy bandwidth); 5 + 2 x 5 of 64, f32 49 and 20; 32 + 2 x 8 of 128 97 and 84 (1.02, 8 pieces
+// 12 heads of 64 58 us then, 35.6 now (0.85 of the copy bandwidth); 5 + 2 x 5 of 64, f32 49 and 20.6; 32 + 2 x 8 of 128 97 and 84 (1.02, 8 pieces
 // 95); 64 tokens of 12 + 2 x 12 heads of 64 2.0 and 1.7.
 constexpr uint32_t AP_THREADS = 256;
 template <int HD> struct ApCfg {

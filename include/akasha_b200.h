@@ -321,7 +321,7 @@ AK_API int ak_kv_read_q8(void* stream, const int8_t* k_pool, const int8_t* v_poo
  *   position to see gives zeros. block_tables int32 [rows, max_blocks_per_seq], entries past a sequence's end are not used; the positions of a
  *   block id outside the pool are left out. scale multiplies q . k.
  *   n_splits: CTAs that share a sequence, as one thread-block cluster; 0 = the library's choice (for
- *   sequences that fill half of their tables), else 1 to 16.
+ *   sequences that fill half of their tables; max_blocks_per_seq far above the blocks in use costs a short call 2 to 6 us), else 1 to 16.
  * Sums, maxima and softmax weights are f32. A query is held as integers of 24 bits (f32) or 16 bits (bf16) of its head's largest value (one under
  * 1e-30 counts as 0); the weights of V have 22 bits, or, for bf16 with more than 4 query rows per kv head (q_len * heads / kv_heads), 11. A weight
  * times its value's scale below 2^-40 (11 bits: 2^-29) of the largest value scale that the query sees may count as 0. */
